@@ -435,6 +435,118 @@ int oga_fp8_quantize_per_head_noalloc(const void* x, int x_dtype, void* q, float
 enum { OGA_ROWS_ADAZERO = 0, OGA_ROWS_ELEMENTWISE = 1 };
 int64_t oga_rows_per_wave(int kind, int64_t batch, int64_t tokens, int64_t cols);
 
+/*
+ * Attention that is trained. No counterpart in the reference, which only
+ * infers: oga_attention's call with what a training step needs, a forward pass
+ * that keeps each row's log-sum-exp and a backward pass that recomputes the
+ * probabilities from it.
+ * q, o, dout, dq [B, Nq, H, D], k, v, dk, dv [B, Nk, Hk, D] bf16, D 64 or 128,
+ * H a multiple of Hk (each key head serves H / Hk query heads); element
+ * strides (batch, token, head) with unit stride along D, multiples of 8, the
+ * token stride below 2^24, 16-byte aligned bases. lse [B, H, Nq] float32.
+ *   S = scale q k^T, lse = log sum exp S, o = exp(S - lse) v,
+ *   dv = P^T dout, dS = P (dout v^T - sum(dout o)), dq = scale dS k,
+ *   dk = scale dS^T q, dk and dv summed over the query heads of a key head.
+ * k_lens (NULL: Nk) [B] int32 on the device: only the first k_lens[b] keys of
+ * sequence b count (taken into 0 .. Nk); what k and v hold behind them is not
+ * read, dk and dv there are 0. With causal != 0 query i sees the keys
+ * j <= i + k_lens[b] - Nq (the last query sees every valid key). A query that
+ * sees no key has o = 0, lse = -inf and no gradient. Scores and sums are
+ * float32, P and dS round to bf16 for the second products, results once.
+ * Nothing is summed by atomics: the same call gives the same bits.
+ * The backward pass needs a 256-byte aligned workspace of
+ * oga_attention_bwd_workspace_bytes(...) bytes on the current device.
+ */
+int oga_attention_lse(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
+                      const void* v, const int64_t v_strides[3], void* o, const int64_t o_strides[3], float* lse,
+                      int64_t batch, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                      float softmax_scale, int causal, const int32_t* k_lens, void* stream);
+int64_t oga_attention_bwd_workspace_bytes(int64_t batch, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads,
+                                          int64_t head_dim);
+int oga_attention_bwd(const void* dout, const int64_t do_strides[3], const void* q, const int64_t q_strides[3],
+                      const void* k, const int64_t k_strides[3], const void* v, const int64_t v_strides[3],
+                      const void* out, const int64_t o_strides[3], const float* lse, void* dq,
+                      const int64_t dq_strides[3], void* dk, const int64_t dk_strides[3], void* dv,
+                      const int64_t dv_strides[3], int64_t batch, int64_t nq, int64_t nk, int64_t heads,
+                      int64_t kv_heads, int64_t head_dim, float softmax_scale, int causal, const int32_t* k_lens,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * RMSNorm of each query and key head with the position rotation in the same
+ * pass (the norms of oga_video_qk_rmsnorm_rope run over the whole row). No
+ * counterpart in the reference. q [B, N, H, D], k [B, N, Hk, D] bf16 or fp16
+ * (x_dtype), D 64, 128 or 256, element strides (batch, token, head) as above
+ * (in place is allowed); Hk 0: q alone. Per head y = Rot(x r w), r =
+ * 1/sqrt(mean(x^2) + eps), w [D] bf16 or float32 (weight_dtype) or NULL for
+ * none. Rot turns the first rotary_dim (a multiple of 16) elements by the
+ * token's angles, in planes (i, i + rotary_dim/2), or with interleaved != 0
+ * (2i, 2i + 1); the others pass. cos, sin [table_len, rotary_dim/2] bf16 or
+ * float32 with row stride cs_stride, row n for token n, or positions[b, n]
+ * (int32, or int64 with positions64 != 0; element strides pos_strides), where
+ * a position outside the table reads its first or last row. norm 0: the
+ * rotation alone; inverse != 0 turns back. float32, rounded once.
+ */
+int oga_head_rmsnorm_rope(int x_dtype, const void* q, const int64_t q_strides[3], const void* k,
+                          const int64_t k_strides[3], const void* q_weight, const void* k_weight, int weight_dtype,
+                          const void* cos, const void* sin, int cs_dtype, int64_t cs_stride, int64_t table_len,
+                          const void* positions, int positions64, const int64_t pos_strides[2], void* q_out,
+                          const int64_t qo_strides[3], void* k_out, const int64_t ko_strides[3], int64_t batch,
+                          int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rotary_dim,
+                          int interleaved, int inverse, int norm, float eps, void* stream);
+
+/*
+ * Backward pass of oga_head_rmsnorm_rope with its norm: from the outputs'
+ * gradients dq_out, dk_out and the inputs, dq, dk and (where not NULL) the
+ * weights' gradients dq_weight, dk_weight [D] in the weights' dtype, summed in
+ * float32 and float64 without atomics. Workspace (16-byte aligned) of
+ * oga_head_rmsnorm_rope_bwd_workspace_bytes(head_dim) bytes where a weight's
+ * gradient is asked for.
+ */
+int64_t oga_head_rmsnorm_rope_bwd_workspace_bytes(int64_t head_dim);
+int oga_head_rmsnorm_rope_bwd(int x_dtype, const void* dq_out, const int64_t dqo_strides[3], const void* dk_out,
+                              const int64_t dko_strides[3], const void* q, const int64_t q_strides[3], const void* k,
+                              const int64_t k_strides[3], const void* q_weight, const void* k_weight,
+                              int weight_dtype, const void* cos, const void* sin, int cs_dtype, int64_t cs_stride,
+                              int64_t table_len, const void* positions, int positions64,
+                              const int64_t pos_strides[2], void* dq, const int64_t dq_strides[3], void* dk,
+                              const int64_t dk_strides[3], void* dq_weight, void* dk_weight, int64_t batch,
+                              int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t rotary_dim,
+                              int interleaved, float eps, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection. No
+ * counterpart in the reference. y, out [rows, n], x [rows, k] bf16 or fp16
+ * with row strides (multiples of 8, 16-byte aligned bases; out may be y);
+ * a [adapters, rank, k], b [adapters, n, rank] contiguous, scale [adapters]
+ * float32 or NULL (1); rank a multiple of 8 up to 128, k and n multiples of 8.
+ * Rows segment_starts[s] .. segment_starts[s + 1] - 1 (int32 [segments + 1],
+ * rising, on the device) take adapter segment_adapters[s] (int32 [segments];
+ * one outside 0 .. adapters - 1 is none):
+ *   out = y + scale b (a x),
+ * and out = y in rows without an adapter and outside all segments. low
+ * [rows, rank] float32 receives scale (a x) of the rows with an adapter; the
+ * backward pass reads it. Starts that do not rise give some rows an undefined
+ * result, within the tensors. Rounded once, at the end.
+ */
+int oga_lora_add(int x_dtype, const void* y, int64_t y_stride, const void* x, int64_t x_stride, const void* a,
+                 const void* b, const float* scale, const int32_t* segment_starts, const int32_t* segment_adapters,
+                 int64_t segments, int64_t adapters, float* low, void* out, int64_t out_stride, int64_t rows,
+                 int64_t k, int64_t n, int64_t rank, void* stream);
+
+/*
+ * Backward pass of oga_lora_add (y's gradient is dy itself): dx [rows, k] =
+ * scale a^T (b^T dy) (0 in rows without an adapter), da and db in a's and b's
+ * layouts, summed over each adapter's rows in float32 in a fixed order (0 for
+ * an adapter without rows). Workspace (256-byte aligned) of
+ * oga_lora_bwd_workspace_bytes(...) bytes on the current device.
+ */
+int64_t oga_lora_bwd_workspace_bytes(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters);
+int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* low,
+                 const void* a, const void* b, const float* scale, const int32_t* segment_starts,
+                 const int32_t* segment_adapters, int64_t segments, int64_t adapters, void* dx, int64_t dx_stride,
+                 void* da, void* db, int64_t rows, int64_t k, int64_t n, int64_t rank, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

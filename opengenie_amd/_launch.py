@@ -1,0 +1,53 @@
+"""What the operators with a row layout of their own share: layouts the kernels
+read, and a call on the tensors' own device and current stream."""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .ltx_ops import _stream
+
+
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """_lib.call(name, *args, stream) on t's device and its current stream."""
+    index = t.get_device()
+    if torch._C._cuda_getDevice() == index:
+        _lib.call(name, *args, _stream(t))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, _stream(t))
+
+
+def bytes_on(t: torch.Tensor, name: str, *args) -> int:
+    """A workspace query, which may go by t's device."""
+    index = t.get_device()
+    if torch._C._cuda_getDevice() == index:
+        return _lib.function(name)(*args)
+    with torch.cuda.device(index):
+        return _lib.function(name)(*args)
+
+
+def heads_layout(t: torch.Tensor, most: int = 1 << 62) -> tuple[torch.Tensor, tuple[int, int, int]]:
+    """t [B, N, H, D] as the kernels read it, and its (batch, token, head)
+    strides: unit stride along D, 16-byte aligned rows, a token stride below
+    `most`; a copy where t is laid out otherwise (an expanded gradient, a
+    transposed view, an odd offset). An axis of one element has stride 0."""
+    b, n, h, d = t.shape
+    sb, sn, sh, sd = t.stride()
+    sb, sn, sh = sb if b > 1 else 0, sn if n > 1 else 0, sh if h > 1 else 0
+    if (sd != 1 and d > 1) or (sb | sn | sh) & 7 or t.data_ptr() & 15 or not 0 <= sn < most:
+        t = t.clone(memory_format=torch.contiguous_format)
+        sb, sn, sh = n * h * d, h * d, d
+    return t, (sb, sn, sh)
+
+
+def rows_layout(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """t (..., C) as rows of C, and the row stride: unit stride along C,
+    16-byte aligned rows; a copy where t is laid out otherwise."""
+    r = t.reshape(-1, t.shape[-1])
+    stride = r.stride(0) if r.shape[0] > 1 else 0
+    if r.stride(1) != 1 or stride & 7 or r.data_ptr() & 15:
+        r = r.clone(memory_format=torch.contiguous_format)
+        stride = r.stride(0)
+    return r, stride

@@ -1,0 +1,980 @@
+// Attention that is trained: a forward pass that keeps each row's log-sum-exp
+// and a backward pass that recomputes the probabilities from it. bf16 in and
+// out, head dimension 64 or 128, shared key/value heads, padded batches
+// (k_lens) and causal masks; float32 softmax and sums.
+//
+//   S = c q k^T,  L_i = log sum_j exp S_ij,  P = exp(S - L),  O = P v
+//   Delta_i = sum_d dO_id O_id,  dP = dO v^T,  dS = P (dP - Delta)
+//   dv = P^T dO,  dq = c dS k,  dk = c dS^T q  (dk, dv: sums over the query
+//   heads that share the key head)
+// P and dS enter the second products rounded to bf16, everything else stays
+// float32 until the results are rounded once.
+//
+// Three kernels share one loop shape: a wave keeps its own rows in registers
+// and walks 64-row tiles of the other side, which LDS-DMA brings into a ring
+// of three tile pairs, two steps ahead (k_attn_lse: 32 queries a wave over K
+// and V; k_attn_dq: the same for dq; k_attn_dkv: 32 keys a wave over Q and dO
+// of all query heads of the group). No sum crosses a workgroup by atomics:
+// recomputing S and dP in both gradient kernels (7 products where 5 would do)
+// costs less than writing and joining partial dq, and results do not depend on
+// the order of workgroups.
+#include "common.h"
+#include "host.h"
+
+namespace oga {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kGT = 64;    // rows of a tile
+constexpr int kGBufs = 3;  // tile pairs in the ring
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct AttnGradArgs {
+  const uint16_t *q, *k, *v, *dout, *out;
+  uint16_t *o, *dq, *dk, *dv;
+  int64_t q_s[3], k_s[3], v_s[3], do_s[3], o_s[3], dq_s[3], dk_s[3], dv_s[3];  // (batch, token, head); unit along D
+  float* lse;          // [B, H, Nq]
+  float* ld;           // [B, H, ceil(Nq / 64)][64 lse2 | 64 Delta] (backward)
+  float* part;         // dk/dv parts: [splits][dk | dv][B, Hk, Nk, D]
+  const int32_t* k_lens;
+  int64_t nq, nk, batch;
+  int heads, kv_heads, group;
+  int blocks;          // query (key) blocks per (batch, head)
+  int causal;
+  int splits;          // parts of a key block's query steps
+  float scale, scale_log2;
+};
+
+OGA_DEVICE int64_t key_count(const AttnGradArgs& a, int64_t b) {
+  return a.k_lens ? min(max((int64_t)a.k_lens[b], (int64_t)0), a.nk) : a.nk;
+}
+
+// The eight XCDs receive workgroups round-robin: renumbered so that each
+// one's are consecutive, the blocks of a head share an L2.
+OGA_DEVICE int64_t xcd_order(uint32_t block, uint32_t grid) {
+  const uint32_t xcd = block & 7, per = grid >> 3, extra = grid & 7;
+  return (int64_t)xcd * per + min(xcd, extra) + (block >> 3);
+}
+
+// ------------------------------------------------------------- LDS tiles
+// Row r of a tile (2 D bytes, D / 8 chunks of 16) keeps chunk c at c ^ sw(r).
+// Two orders, by how the kernel reads: 32-row fragments (32x32x16 MFMA) with
+// transposing reads of 4 rows x 64 bytes, or 16-row fragments (16x16x32) with
+// transposing reads of 8 rows x 32 bytes; each read's lanes then cover all
+// banks once.
+template <int D>
+constexpr int sw32(int r) {
+  return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+}
+template <int D>
+constexpr int sw16(int r) {
+  return D == 128 ? ((r & 7) << 1) | ((r >> 3) & 1) : (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
+}
+
+template <int OFF>
+OGA_DEVICE bf16x8 rd_b128(uint32_t addr) {
+  static_assert(OFF >= 0 && OFF < 2 * 65536, "LDS offset");
+  uint4 v;
+  if constexpr (OFF >= 65536)
+    asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(addr + 65536u), "i"(OFF - 65536));
+  else
+    asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "i"(OFF));
+  return __builtin_bit_cast(bf16x8, v);
+}
+template <int OFF>
+OGA_DEVICE u32x2 rd_tr16(uint32_t addr) {
+  static_assert(OFF >= 0 && OFF < 2 * 65536, "LDS offset");
+  u32x2 v;
+  if constexpr (OFF >= 65536)
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(v) : "v"(addr + 65536u), "i"(OFF - 65536));
+  else
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "i"(OFF));
+  return v;
+}
+// An LDS address made where it is used: the compiler would otherwise keep the
+// dozens of addresses that differ in a few bits in registers over the loop.
+OGA_DEVICE uint32_t here(uint32_t addr, uint32_t add) {
+  addr += add;
+  asm volatile("" : "+v"(addr));
+  return addr;
+}
+#define GRAD_LGKM(N, ...) asm volatile("s_waitcnt lgkmcnt(" #N ")" : __VA_ARGS__)
+
+OGA_DEVICE bf16x8 frag2(const u32x2& a, const u32x2& b) {
+  const uint4 u = {a[0], a[1], b[0], b[1]};
+  return __builtin_bit_cast(bf16x8, u);
+}
+OGA_DEVICE f32x16 mfma32(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+OGA_DEVICE f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// LDS-DMA of a 64-row tile by W waves: instruction i of wave w fills 1 KiB.
+// Rows past the last one (`rows` of them exist) read the last one again.
+// A source is a uniform base and a 32-bit offset made anew for each tile from
+// the lane number: kept over the loop, the offsets would be the registers that
+// k_attn_dkv does not have.
+template <int D, int W, bool S16>
+struct TileDma {
+  static constexpr int kCh = D / 8, kRpi = 64 / kCh, kDI = kGT / kRpi / W;
+  static_assert(kDI >= 1, "waves");
+  static OGA_DEVICE void send(const uint16_t* base, uint32_t row_stride, int rows, char* lds, int wv, int lane) {
+    asm volatile("" : "+v"(lane));
+#pragma unroll
+    for (int i = 0; i < kDI; ++i) {
+      const int row = (wv * kDI + i) * kRpi + lane / kCh;
+      const int chunk = (lane % kCh) ^ (S16 ? sw16<D>(row) : sw32<D>(row));
+      const uint32_t off = __umul24((uint32_t)min(row, rows - 1), row_stride) * 2 + chunk * 16;
+      __builtin_amdgcn_global_load_lds((const void*)((const char*)base + off),
+                                       (lds_void*)(lds + (wv * kDI + i) * 1024), 16, 0, 0);
+    }
+  }
+};
+
+// One step of a kernel's tile loop in ring slot SLOT: wait until this wave's
+// DMA of the step has landed (that of the next step, AHEAD instructions, may
+// be in flight), then for every wave. A bare barrier: a fence would drain the
+// DMA sent ahead, and the LDS reads are inline assembly.
+template <int AHEAD>
+OGA_DEVICE void ring_wait() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(AHEAD) : "memory");
+  asm volatile("s_barrier" ::: "memory");
+}
+
+OGA_DEVICE float max_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+OGA_DEVICE float sum_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---------------------------------------------------------------- forward
+// W waves of 32 queries. S^T = K Q^T in 32 x 32 blocks (lane l: query l % 32,
+// keys 8g + 4 (l / 32) + r), online softmax in base 2 with the running max
+// moved only when a score passes it by 8 (P stays below 2^8), O^T += V^T P^T.
+template <int D, int W, bool CAUSAL>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attn_lse(AttnGradArgs a) {
+  constexpr int kTile = kGT * D * 2, kPair = 2 * kTile, NS = D / 16, ND = D / 32;
+  typedef TileDma<D, W, false> Dma;
+  __shared__ uint4 smem[kGBufs * kPair / 16];
+  const int lane = threadIdx.x & 63;
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int64_t wg = xcd_order(blockIdx.x, gridDim.x);
+  int qb = (int)(wg % a.blocks);
+  if (CAUSAL) qb = a.blocks - 1 - qb;  // the longest first
+  const int64_t bh = wg / a.blocks;
+  const int h = (int)(bh % a.heads);
+  const int64_t b = bh / a.heads;
+  const int hk = h / a.group;
+  const int hl = lane >> 5, ql = lane & 31;
+  const int64_t q0 = (int64_t)qb * 32 * W + wv * 32;
+  const int64_t nkb = key_count(a, b);
+  const int64_t shift = nkb - a.nq;  // causal: query i sees keys <= i + shift
+  int64_t kend = nkb;
+  if (CAUSAL) kend = min(nkb, max((int64_t)0, min((int64_t)(qb + 1) * 32 * W, a.nq) + shift));
+  const int nsteps = (int)((kend + kGT - 1) / kGT);
+
+  bf16x8 qf[NS];
+  {
+    const uint16_t* qr = a.q + b * a.q_s[0] + min(q0 + ql, a.nq - 1) * a.q_s[1] + (int64_t)h * a.q_s[2];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] = __builtin_bit_cast(bf16x8, *(const uint4*)(qr + 16 * s + 8 * hl));
+  }
+  f32x16 o[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+  float m_run = -INFINITY, l_run = 0.0f;
+
+  const uint16_t* kb = a.k + b * a.k_s[0] + (int64_t)hk * a.k_s[2];
+  const uint16_t* vb = a.v + b * a.v_s[0] + (int64_t)hk * a.v_s[2];
+  char* const lds = (char*)smem;
+  auto dma = [&](int st, int slot) {
+    const int64_t key0 = (int64_t)st * kGT;
+    const int rows = (int)min((int64_t)kGT, nkb - key0);
+    Dma::send(kb + key0 * a.k_s[1], (uint32_t)a.k_s[1], rows, lds + slot * kPair, wv, lane);
+    Dma::send(vb + key0 * a.v_s[1], (uint32_t)a.v_s[1], rows, lds + slot * kPair + kTile, wv, lane);
+  };
+
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)smem;
+  const uint32_t ka = lds0 + ql * (2 * D) + ((hl ^ sw32<D>(ql)) << 4);
+  const int a4 = lane & 3, j4 = (lane & 15) >> 2, g2 = (lane >> 4) & 1;
+  const uint32_t va = lds0 + kTile + (4 * hl + j4) * (2 * D) +
+                      (((2 * g2 + (a4 >> 1)) ^ sw32<D>(4 * hl + j4)) << 4) + (a4 & 1) * 8;
+
+  auto step = [&](auto slot_c, int st) {
+    constexpr int SLOT = decltype(slot_c)::value, BASE = SLOT * kPair;
+    ring_wait<2 * Dma::kDI>();
+    dma(min(st + 2, nsteps - 1), (SLOT + 2) % kGBufs);
+    f32x16 s[2];
+    auto block = [&](auto j_c) {
+      constexpr int OFF = BASE + 32 * 2 * D * decltype(j_c)::value;
+      bf16x8 f[NS];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) f[i] = rd_b128<OFF>(ka ^ (i << 5));
+      if constexpr (NS == 8)
+        GRAD_LGKM(0, "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]), "+v"(f[4]), "+v"(f[5]), "+v"(f[6]), "+v"(f[7]));
+      else
+        GRAD_LGKM(0, "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]));
+      f32x16 acc;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) acc = mfma32(f[i], qf[i], acc);
+      return acc;
+    };
+    s[0] = block(IC<0>{});
+    s[1] = block(IC<1>{});
+    // V^T of 16-key chunk C: reads for each 32-wide d-block, both 8-key halves
+    auto read_v = [&](auto c_c, u32x2(&vr)[2 * ND]) {
+      constexpr int OFF = BASE + 16 * 2 * D * decltype(c_c)::value;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        vr[2 * d] = rd_tr16<OFF>(va ^ (d << 6));
+        vr[2 * d + 1] = rd_tr16<OFF + 8 * 2 * D>(va ^ ((d << 6) | 32));
+      }
+    };
+    u32x2 v0[2 * ND], v1[2 * ND];
+    read_v(IC<0>{}, v0);
+    const int64_t key0 = (int64_t)st * kGT;
+    // keys at or past `limit` (relative to this lane's first) are hidden
+    const int64_t lim64 = CAUSAL ? min(nkb, q0 + ql + shift + 1) - key0 : nkb - key0;
+    if (CAUSAL ? key0 + kGT > min(nkb, q0 + shift + 1) : lim64 < kGT) {
+      const int lim = (int)max(min(lim64, (int64_t)kGT), (int64_t)-kGT) - 4 * hl;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (32 * j + 8 * (e >> 2) + (e & 3) >= lim) s[j][e] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = (j == 0 ? 1 : 0); e < 16; ++e) mx = __builtin_fmaxf(mx, s[j][e]);
+    const float ms = max_halves(mx) * a.scale_log2;
+    if (__any(ms > m_run + 8.0f)) {
+      const float m_new = __builtin_fmaxf(m_run, ms);
+      // a row that has seen no key yet keeps O = l = 0 (and m = -inf)
+      const float alpha = __builtin_amdgcn_exp2f(m_run - (m_new == -INFINITY ? 0.0f : m_new));
+      l_run *= alpha;
+      m_run = m_new;
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
+    }
+    const float nm = m_run == -INFINITY ? 0.0f : -m_run;
+    uint32_t pb[2][8];
+    float ps0 = 0.0f, ps1 = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][e], a.scale_log2, nm));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][e + 1], a.scale_log2, nm));
+        ps0 += p0;
+        ps1 += p1;
+        pb[j][e >> 1] = pack_bf16(p0, p1);
+      }
+    l_run += ps0 + ps1;
+    auto pv = [&](auto c_c, u32x2(&cur)[2 * ND], u32x2(&nxt)[2 * ND]) {
+      constexpr int C = decltype(c_c)::value;
+      if constexpr (C < 3) read_v(IC<(C + 1) & 3>{}, nxt);
+      if constexpr (ND == 4) {
+        if constexpr (C < 3)
+          GRAD_LGKM(8, "+v"(cur[0]), "+v"(cur[1]), "+v"(cur[2]), "+v"(cur[3]), "+v"(cur[4]), "+v"(cur[5]), "+v"(cur[6]),
+                    "+v"(cur[7]));
+        else
+          GRAD_LGKM(0, "+v"(cur[0]), "+v"(cur[1]), "+v"(cur[2]), "+v"(cur[3]), "+v"(cur[4]), "+v"(cur[5]), "+v"(cur[6]),
+                    "+v"(cur[7]));
+      } else {
+        if constexpr (C < 3)
+          GRAD_LGKM(4, "+v"(cur[0]), "+v"(cur[1]), "+v"(cur[2]), "+v"(cur[3]));
+        else
+          GRAD_LGKM(0, "+v"(cur[0]), "+v"(cur[1]), "+v"(cur[2]), "+v"(cur[3]));
+      }
+      const uint32_t* pw = &pb[C >> 1][4 * (C & 1)];
+      const uint4 pu = {pw[0], pw[1], pw[2], pw[3]};
+#pragma unroll
+      for (int d = 0; d < ND; ++d) o[d] = mfma32(frag2(cur[2 * d], cur[2 * d + 1]), __builtin_bit_cast(bf16x8, pu), o[d]);
+    };
+    pv(IC<0>{}, v0, v1);
+    pv(IC<1>{}, v1, v0);
+    pv(IC<2>{}, v0, v1);
+    pv(IC<3>{}, v1, v0);
+  };
+
+  if (nsteps > 0) {  // (uniform over the workgroup)
+    dma(0, 0);
+    dma(min(1, nsteps - 1), 1);
+    for (int st = 0; st < nsteps; st += 3) {
+      step(IC<0>{}, st);
+      if (st + 1 < nsteps) step(IC<1>{}, st + 1);
+      if (st + 2 < nsteps) step(IC<2>{}, st + 2);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+  const float l = sum_halves(l_run);
+  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // no key: 0; NaN stays
+  const int64_t qi = q0 + ql;
+  if (hl == 0 && qi < a.nq)
+    a.lse[bh * a.nq + qi] = l == 0.0f ? -INFINITY : m_run * kLn2 + logf(l);
+  // Through the wave's own LDS (the tiles are done with), so that each store
+  // writes whole rows: 16-byte chunk c of row r sits at c ^ (r % (D / 8)).
+  __syncthreads();
+  char* const ot = lds + wv * 32 * 2 * D;
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      uint2 w;
+      w.x = pack_bf16(o[d][4 * g] * inv, o[d][4 * g + 1] * inv);
+      w.y = pack_bf16(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv);
+      *(uint2*)(ot + ql * 2 * D + (((4 * d + g) ^ (ql % (D / 8))) << 4) + 8 * hl) = w;
+    }
+  __syncthreads();
+  constexpr int kLpr = D / 8, kRows = 64 / kLpr;  // lanes a row, rows a store
+  const int oc = lane % kLpr;
+  uint16_t* ob = a.o + b * a.o_s[0] + (int64_t)h * a.o_s[2] + 8 * oc;
+#pragma unroll
+  for (int it = 0; it < 32 / kRows; ++it) {
+    const int r = kRows * it + lane / kLpr;
+    const uint4 w = *(const uint4*)(ot + r * 2 * D + ((oc ^ (r % kLpr)) << 4));
+    if (q0 + r < a.nq) *(uint4*)(ob + (q0 + r) * a.o_s[1]) = w;
+  }
+}
+
+// --------------------------------------------------- Delta and base-2 lse
+// D / 8 lanes a row of O and dO; rows behind the last query (up to the tile's
+// 64) and rows that saw no key get lse2 = +inf, so that their P is 0.
+template <int D>
+__global__ __launch_bounds__(256) void k_attn_delta(AttnGradArgs a) {
+  constexpr int kLpr = D / 8;
+  const int64_t nqp = (a.nq + kGT - 1) / kGT * kGT;
+  const int64_t row = (int64_t)blockIdx.x * (256 / kLpr) + threadIdx.x / kLpr;  // (b, n, h), h fastest
+  if (row >= a.batch * nqp * a.heads) return;
+  const int c = threadIdx.x % kLpr;
+  const int64_t bn = row / a.heads;
+  const int h = (int)(row - bn * a.heads);
+  const int64_t b = bn / nqp, n = bn - b * nqp;
+  float delta = 0.0f, lse2 = INFINITY;
+  if (n < a.nq) {
+    float f[8], g[8];
+    unpack8(*(const uint4*)(a.out + b * a.o_s[0] + n * a.o_s[1] + (int64_t)h * a.o_s[2] + 8 * c), f);
+    unpack8(*(const uint4*)(a.dout + b * a.do_s[0] + n * a.do_s[1] + (int64_t)h * a.do_s[2] + 8 * c), g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) delta = fmaf(f[i], g[i], delta);
+    const float l = a.lse[(b * a.heads + h) * a.nq + n];
+    lse2 = l == -INFINITY ? INFINITY : l * kLog2e;
+  }
+#pragma unroll
+  for (int m = 1; m < kLpr; m <<= 1) delta += __shfl_xor(delta, m, 64);
+  if (c == 0) {
+    float* t = a.ld + ((b * a.heads + h) * (nqp / kGT) + n / kGT) * 128 + n % kGT;
+    t[0] = lse2;
+    t[64] = delta;
+  }
+}
+
+// --------------------------------------------------------------------- dq
+// 8 waves of 32 queries over tiles of 64 keys. S^T = K Q^T and dP^T = V dO^T
+// in 16 x 16 blocks (lane l: query l % 16, keys 4 (l / 16) + r), so a lane's
+// lse and Delta are two numbers; dq^T += K^T dS^T with K^T by transposing
+// reads, whose 32 keys' order (4 (l / 16) + r of two 16-key blocks) is that of
+// the blocks' accumulators. 16x16x32 MFMAs draw less power than 32x32x16 at
+// the same rate, and no row maximum is needed here.
+constexpr int kGW = 8;
+template <int D, bool CAUSAL>
+__global__ __launch_bounds__(64 * kGW) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attn_dq(AttnGradArgs a) {
+  constexpr int kTile = kGT * D * 2, kPair = 2 * kTile, NS = D / 32, ND = D / 16;
+  typedef TileDma<D, kGW, true> Dma;
+  __shared__ uint4 smem[kGBufs * kPair / 16];
+  const int lane = threadIdx.x & 63;
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int64_t wg = xcd_order(blockIdx.x, gridDim.x);
+  int qb = (int)(wg % a.blocks);
+  if (CAUSAL) qb = a.blocks - 1 - qb;
+  const int64_t bh = wg / a.blocks;
+  const int h = (int)(bh % a.heads);
+  const int64_t b = bh / a.heads;
+  const int hk = h / a.group;
+  const int c16 = lane & 15, kg = lane >> 4;
+  const int64_t q0 = (int64_t)qb * 32 * kGW + wv * 32;
+  const int64_t nkb = key_count(a, b);
+  const int64_t shift = nkb - a.nq;
+  int64_t kend = nkb;
+  if (CAUSAL) kend = min(nkb, max((int64_t)0, min((int64_t)(qb + 1) * 32 * kGW, a.nq) + shift));
+  const int nsteps = (int)((kend + kGT - 1) / kGT);
+
+  bf16x8 qf[2][NS], gf[2][NS];  // Q and dO, B operands: query 16 i + c16, d = 32 s + 8 kg ..
+  float lse2[2], delta[2];
+  const int64_t nqt = (a.nq + kGT - 1) / kGT;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t qi = min(q0 + 16 * i + c16, a.nq - 1);
+    const uint16_t* qr = a.q + b * a.q_s[0] + qi * a.q_s[1] + (int64_t)h * a.q_s[2] + 8 * kg;
+    const uint16_t* gr = a.dout + b * a.do_s[0] + qi * a.do_s[1] + (int64_t)h * a.do_s[2] + 8 * kg;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      qf[i][s] = __builtin_bit_cast(bf16x8, *(const uint4*)(qr + 32 * s));
+      gf[i][s] = __builtin_bit_cast(bf16x8, *(const uint4*)(gr + 32 * s));
+    }
+    const float* t = a.ld + (bh * nqt + qi / kGT) * 128 + qi % kGT;
+    lse2[i] = t[0];
+    delta[i] = t[64];
+  }
+  f32x4 acc[ND][2];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) acc[d][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const uint16_t* kb = a.k + b * a.k_s[0] + (int64_t)hk * a.k_s[2];
+  const uint16_t* vb = a.v + b * a.v_s[0] + (int64_t)hk * a.v_s[2];
+  char* const lds = (char*)smem;
+  auto dma = [&](int st, int slot) {
+    const int64_t key0 = (int64_t)st * kGT;
+    const int rows = (int)min((int64_t)kGT, nkb - key0);
+    Dma::send(kb + key0 * a.k_s[1], (uint32_t)a.k_s[1], rows, lds + slot * kPair, wv, lane);
+    Dma::send(vb + key0 * a.v_s[1], (uint32_t)a.v_s[1], rows, lds + slot * kPair + kTile, wv, lane);
+  };
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)smem;
+  const uint32_t ra = lds0 + c16 * (2 * D) + ((kg ^ sw16<D>(c16)) << 4);
+  const int a4 = lane & 3, j4 = (lane & 15) >> 2;
+  const uint32_t ta = lds0 + (4 * kg + j4) * (2 * D) + (((a4 >> 1) ^ sw16<D>(4 * kg + j4)) << 4) + (a4 & 1) * 8;
+
+  auto step = [&](uint32_t base, int slot2, int st) {
+    ring_wait<2 * Dma::kDI>();
+    dma(min(st + 2, nsteps - 1), slot2);
+    const int64_t key0 = (int64_t)st * kGT;
+    const bool edge = CAUSAL ? key0 + kGT > min(nkb, q0 + shift + 1) : key0 + kGT > nkb;
+    auto half = [&](auto j_c) {  // keys 32 j .. + 31 of the tile
+      constexpr int OFF = 32 * 2 * D * decltype(j_c)::value;
+      uint32_t ds[2][4];  // dS^T, B operand of dq: query block i
+      auto block = [&](auto u_c) {  // keys 16 u .. + 15 of these
+        constexpr int U = decltype(u_c)::value;
+        const uint32_t r0 = here(ra, base);
+        f32x4 s[2], g[2];
+        bf16x8 kf[NS], vf[NS];
+#pragma unroll
+        for (int x = 0; x < NS; ++x) kf[x] = rd_b128<OFF + 16 * 2 * D * U>(r0 ^ (x << 6));
+#pragma unroll
+        for (int x = 0; x < NS; ++x) vf[x] = rd_b128<OFF + 16 * 2 * D * U + kTile>(r0 ^ (x << 6));
+        if constexpr (NS == 4)
+          GRAD_LGKM(4, "+v"(kf[0]), "+v"(kf[1]), "+v"(kf[2]), "+v"(kf[3]));
+        else
+          GRAD_LGKM(2, "+v"(kf[0]), "+v"(kf[1]));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, g[i] = s[i];
+#pragma unroll
+        for (int x = 0; x < NS; ++x)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) s[i] = mfma16(kf[x], qf[i][x], s[i]);
+        if constexpr (NS == 4)
+          GRAD_LGKM(0, "+v"(vf[0]), "+v"(vf[1]), "+v"(vf[2]), "+v"(vf[3]));
+        else
+          GRAD_LGKM(0, "+v"(vf[0]), "+v"(vf[1]));
+#pragma unroll
+        for (int x = 0; x < NS; ++x)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) g[i] = mfma16(vf[x], gf[i][x], g[i]);
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int64_t lim64 = (CAUSAL ? min(nkb, q0 + 16 * i + c16 + shift + 1) : nkb) - key0;
+            const int lim = (int)max(min(lim64, (int64_t)kGT), (int64_t)-kGT) - 4 * kg - 32 * decltype(j_c)::value - 16 * U;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (r >= lim) s[i][r] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float d[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], a.scale_log2, -lse2[i]));
+            d[r] = p * (g[i][r] - delta[i]);
+          }
+          ds[i][2 * U] = pack_bf16(d[0], d[1]);
+          ds[i][2 * U + 1] = pack_bf16(d[2], d[3]);
+        }
+      };
+      block(IC<0>{});
+      block(IC<1>{});
+      bf16x8 df[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint4 u = {ds[i][0], ds[i][1], ds[i][2], ds[i][3]};
+        df[i] = __builtin_bit_cast(bf16x8, u);
+      }
+#pragma unroll
+      for (int d = 0; d < ND; d += 4) {
+        const uint32_t w0 = here(ta, base);
+        u32x2 t[8];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          t[2 * x] = rd_tr16<OFF>(w0 ^ ((d + x) << 5));
+          t[2 * x + 1] = rd_tr16<OFF + 16 * 2 * D>(w0 ^ ((d + x) << 5));
+        }
+        GRAD_LGKM(0, "+v"(t[0]), "+v"(t[1]), "+v"(t[2]), "+v"(t[3]), "+v"(t[4]), "+v"(t[5]), "+v"(t[6]), "+v"(t[7]));
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) acc[d + x][i] = mfma16(frag2(t[2 * x], t[2 * x + 1]), df[i], acc[d + x][i]);
+      }
+    };
+    half(IC<0>{});
+    half(IC<1>{});
+  };
+  if (nsteps > 0) {
+    dma(0, 0);
+    dma(min(1, nsteps - 1), 1);
+    int slot = 0;
+    for (int st = 0; st < nsteps; ++st) {
+      step(slot * kPair, slot == 0 ? 2 : slot - 1, st);
+      slot = slot == 2 ? 0 : slot + 1;
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  // lane: query 16 i + c16, d = 16 db + 4 kg .. + 3
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t qi = q0 + 16 * i + c16;
+    if (qi >= a.nq) continue;
+    uint16_t* o = a.dq + b * a.dq_s[0] + qi * a.dq_s[1] + (int64_t)h * a.dq_s[2] + 4 * kg;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      *(uint2*)(o + 16 * d) = make_uint2(pack_bf16(acc[d][i][0] * a.scale, acc[d][i][1] * a.scale),
+                                         pack_bf16(acc[d][i][2] * a.scale, acc[d][i][3] * a.scale));
+  }
+}
+
+// ------------------------------------------------------------- dk and dv
+// 8 waves of 32 keys (K and V in registers as B operands) over tiles of 64
+// queries of every query head of the group. S = Q K^T and dP = dO V^T in
+// 16 x 16 blocks (lane l: key l % 16, queries 4 (l / 16) + r), whose lse and
+// Delta come from LDS, four queries a read; dv^T += dO^T P and dk^T += Q^T dS
+// with the transposed tiles by transposing reads.
+template <int D>
+struct DkvShape {
+  static constexpr int kW = 8;   // waves
+  static constexpr int kKB = 2;  // 16-key blocks per wave
+  static constexpr int kKeys = 16 * kW * kKB;   // keys per workgroup
+};
+template <int D, bool CAUSAL>
+__global__ __launch_bounds__(64 * DkvShape<D>::kW) __attribute__((amdgpu_waves_per_eu(DkvShape<D>::kW / 4, DkvShape<D>::kW / 4))) void k_attn_dkv(AttnGradArgs a) {
+  constexpr int kTile = kGT * D * 2, kPair = 2 * kTile + 512, NS = D / 32, ND = D / 16;
+  constexpr int W = DkvShape<D>::kW, KB = DkvShape<D>::kKB, kKeys = DkvShape<D>::kKeys;
+  typedef TileDma<D, W, true> Dma;
+  __shared__ uint4 smem[kGBufs * kPair / 16];
+  const int lane = threadIdx.x & 63;
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int64_t unit = xcd_order(blockIdx.x, gridDim.x);
+  const int part = (int)(unit % a.splits);
+  const int64_t wg = unit / a.splits;
+  const int kblk = (int)(wg % a.blocks);
+  const int64_t bh = wg / a.blocks;
+  const int hk = (int)(bh % a.kv_heads);
+  const int64_t b = bh / a.kv_heads;
+  const int c16 = lane & 15, kg = lane >> 4;
+  const int64_t kblk0 = (int64_t)kblk * kKeys, k0 = kblk0 + wv * 16 * KB;
+  const int64_t nkb = key_count(a, b);
+  const int64_t shift = nkb - a.nq;
+  const int nqt = (int)((a.nq + kGT - 1) / kGT);
+  // Query tiles t0 .. nqt - 1 of each head; this part takes steps s0 .. s1 - 1
+  // of the group's.
+  int t0 = 0;
+  if (CAUSAL) t0 = (int)min((int64_t)nqt, max((int64_t)0, kblk0 - shift) / kGT);
+  if (kblk0 >= nkb) t0 = nqt;
+  const int per = nqt - t0;
+  const int64_t all = (int64_t)per * a.group;
+  const int s0 = (int)(all * part / a.splits), s1 = (int)(all * (part + 1) / a.splits);
+
+  bf16x8 kf[KB][NS], vf[KB][NS];
+  f32x4 dk[ND][KB], dv[ND][KB];
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int i = 0; i < KB; ++i) dk[d][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, dv[d][i] = dk[d][i];
+
+  if (s1 > s0) {
+#pragma unroll
+    for (int i = 0; i < KB; ++i) {
+      const int64_t ki = min(k0 + 16 * i + c16, nkb - 1);
+      const uint16_t* kr = a.k + b * a.k_s[0] + ki * a.k_s[1] + (int64_t)hk * a.k_s[2] + 8 * kg;
+      const uint16_t* vr = a.v + b * a.v_s[0] + ki * a.v_s[1] + (int64_t)hk * a.v_s[2] + 8 * kg;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        kf[i][s] = __builtin_bit_cast(bf16x8, *(const uint4*)(kr + 32 * s));
+        vf[i][s] = __builtin_bit_cast(bf16x8, *(const uint4*)(vr + 32 * s));
+      }
+    }
+    const uint16_t* qbase = a.q + b * a.q_s[0] + (int64_t)hk * a.group * a.q_s[2];
+    const uint16_t* gbase = a.dout + b * a.do_s[0] + (int64_t)hk * a.group * a.do_s[2];
+    const float* lbase = a.ld + (b * a.heads + (int64_t)hk * a.group) * nqt * 128;
+    char* const lds = (char*)smem;
+    // The next step to send: its head of the group and query tile (the last
+    // one again past the end).
+    int send_s = s0, send_g = s0 / per, send_t = t0 + s0 % per;
+    auto dma = [&](int slot) {
+      const int g = send_g, t = send_t;
+      if (send_s + 1 < s1) {
+        ++send_s;
+        if (++send_t == nqt) send_t = t0, ++send_g;
+      }
+      const int64_t q0 = (int64_t)t * kGT;
+      const int rows = (int)min((int64_t)kGT, a.nq - q0);
+      char* const at = lds + slot * kPair;
+      Dma::send(qbase + g * a.q_s[2] + q0 * a.q_s[1], (uint32_t)a.q_s[1], rows, at, wv, lane);
+      Dma::send(gbase + g * a.do_s[2] + q0 * a.do_s[1], (uint32_t)a.do_s[1], rows, at + kTile, wv, lane);
+      // lse2 and Delta, 256 bytes each: even waves the one, odd waves the other
+      int l = lane;
+      asm volatile("" : "+v"(l));
+      const uint32_t off = 4 * l;
+      __builtin_amdgcn_global_load_lds(
+          (const void*)((const char*)(lbase + ((int64_t)g * nqt + t) * 128 + (wv & 1) * 64) + off),
+          (lds_void*)(at + 2 * kTile + (wv & 1) * 256), 4, 0, 0);
+    };
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)smem;
+    const uint32_t ra = lds0 + c16 * (2 * D) + ((kg ^ sw16<D>(c16)) << 4);
+    const int a4 = lane & 3, j4 = (lane & 15) >> 2;
+    const uint32_t ta = lds0 + (4 * kg + j4) * (2 * D) + (((a4 >> 1) ^ sw16<D>(4 * kg + j4)) << 4) + (a4 & 1) * 8;
+
+    auto step = [&](uint32_t base, int slot2, int first) {
+      ring_wait<2 * Dma::kDI + 1>();
+      dma(slot2);
+      auto half = [&](auto j_c) {  // queries 32 j .. + 31 of the tile
+        constexpr int J = decltype(j_c)::value, OFF = 32 * 2 * D * J;
+        uint32_t pp[KB][4], ds[KB][4];  // P and dS, B operands: key block i
+        auto block = [&](auto u_c) {  // queries 16 u .. + 15 of these
+          constexpr int U = decltype(u_c)::value;
+          const uint32_t r0 = here(ra, base);
+          constexpr int OQ = OFF + 16 * 2 * D * U, OG = OQ + kTile, OL = (32 * J + 16 * U) * 4;
+          f32x4 s[KB], g[KB];
+#pragma unroll
+          for (int i = 0; i < KB; ++i) s[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, g[i] = s[i];
+          // two pairs of fragments in flight, each read under the other's MFMAs
+          bf16x8 x0, x1, y0, y1;
+          auto mul = [&](f32x4(&c)[KB], const bf16x8& u, const bf16x8& v, const bf16x8(&w)[KB][NS], auto n_c) {
+            constexpr int N = decltype(n_c)::value;
+#pragma unroll
+            for (int i = 0; i < KB; ++i) c[i] = mfma16(u, w[i][N], c[i]);
+#pragma unroll
+            for (int i = 0; i < KB; ++i) c[i] = mfma16(v, w[i][N + 1], c[i]);
+          };
+          x0 = rd_b128<OQ>(r0);
+          x1 = rd_b128<OQ>(r0 ^ 64);
+          if constexpr (NS == 4) {
+            y0 = rd_b128<OQ>(r0 ^ 128);
+            y1 = rd_b128<OQ>(r0 ^ 192);
+            GRAD_LGKM(2, "+v"(x0), "+v"(x1));
+            mul(s, x0, x1, kf, IC<0>{});
+            x0 = rd_b128<OG>(r0);
+            x1 = rd_b128<OG>(r0 ^ 64);
+            GRAD_LGKM(2, "+v"(y0), "+v"(y1));
+            mul(s, y0, y1, kf, IC<2 % NS>{});
+            y0 = rd_b128<OG>(r0 ^ 128);
+            y1 = rd_b128<OG>(r0 ^ 192);
+            GRAD_LGKM(2, "+v"(x0), "+v"(x1));
+            mul(g, x0, x1, vf, IC<0>{});
+            const uint32_t l0 = (here(lane, 0) & ~15u) + lds0 + 2 * kTile + base;  // 16 kg
+            x0 = rd_b128<OL>(l0);
+            x1 = rd_b128<OL + 256>(l0);
+            GRAD_LGKM(2, "+v"(y0), "+v"(y1));
+            mul(g, y0, y1, vf, IC<2 % NS>{});
+          } else {
+            y0 = rd_b128<OG>(r0);
+            y1 = rd_b128<OG>(r0 ^ 64);
+            GRAD_LGKM(2, "+v"(x0), "+v"(x1));
+            mul(s, x0, x1, kf, IC<0>{});
+            const uint32_t l0 = (here(lane, 0) & ~15u) + lds0 + 2 * kTile + base;  // 16 kg
+            x0 = rd_b128<OL>(l0);
+            x1 = rd_b128<OL + 256>(l0);
+            GRAD_LGKM(2, "+v"(y0), "+v"(y1));
+            mul(g, y0, y1, vf, IC<0>{});
+          }
+          GRAD_LGKM(0, "+v"(x0), "+v"(x1));
+          const f32x4 lse2 = __builtin_bit_cast(f32x4, x0), delta = __builtin_bit_cast(f32x4, x1);
+          if constexpr (CAUSAL) {
+#pragma unroll
+            for (int i = 0; i < KB; ++i) {
+              // compared in every tile: behind a uniform branch the scores cost
+              // more registers than there are
+              const int l = (int)here(lane, 0);
+              const int low = first + 16 * i + (l & 15) - 4 * (l >> 4) - 32 * J - 16 * U;
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (r < low) s[i][r] = -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < KB; ++i) {
+            float p[4], d[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], a.scale_log2, -lse2[r]));
+              d[r] = p[r] * (g[i][r] - delta[r]);
+            }
+            pp[i][2 * U] = pack_bf16(p[0], p[1]);
+            pp[i][2 * U + 1] = pack_bf16(p[2], p[3]);
+            ds[i][2 * U] = pack_bf16(d[0], d[1]);
+            ds[i][2 * U + 1] = pack_bf16(d[2], d[3]);
+          }
+        };
+        __builtin_amdgcn_sched_barrier(0);
+        block(IC<0>{});
+        __builtin_amdgcn_sched_barrier(0);
+        block(IC<1>{});
+        __builtin_amdgcn_sched_barrier(0);
+        bf16x8 pf[KB], df[KB];
+#pragma unroll
+        for (int i = 0; i < KB; ++i) {
+          const uint4 u = {pp[i][0], pp[i][1], pp[i][2], pp[i][3]}, w = {ds[i][0], ds[i][1], ds[i][2], ds[i][3]};
+          pf[i] = __builtin_bit_cast(bf16x8, u);
+          df[i] = __builtin_bit_cast(bf16x8, w);
+        }
+#pragma unroll
+        for (int d = 0; d < ND; d += 2) {
+          const uint32_t w0 = here(ta, base);
+          u32x2 x[4], y[4];  // dO^T and Q^T of two 16-wide d-blocks
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            x[2 * z] = rd_tr16<OFF + kTile>(w0 ^ ((d + z) << 5));
+            x[2 * z + 1] = rd_tr16<OFF + kTile + 16 * 2 * D>(w0 ^ ((d + z) << 5));
+          }
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            y[2 * z] = rd_tr16<OFF>(w0 ^ ((d + z) << 5));
+            y[2 * z + 1] = rd_tr16<OFF + 16 * 2 * D>(w0 ^ ((d + z) << 5));
+          }
+          GRAD_LGKM(4, "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]));
+#pragma unroll
+          for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int i = 0; i < KB; ++i) dv[d + z][i] = mfma16(frag2(x[2 * z], x[2 * z + 1]), pf[i], dv[d + z][i]);
+          GRAD_LGKM(0, "+v"(y[0]), "+v"(y[1]), "+v"(y[2]), "+v"(y[3]));
+#pragma unroll
+          for (int z = 0; z < 2; ++z)
+#pragma unroll
+            for (int i = 0; i < KB; ++i) dk[d + z][i] = mfma16(frag2(y[2 * z], y[2 * z + 1]), df[i], dk[d + z][i]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      half(IC<0>{});
+      half(IC<1>{});
+    };
+    int t = t0 + s0 % per;  // this step's query tile
+    dma(0);
+    dma(1);
+    int slot = 0;
+    for (int st = s0; st < s1; ++st) {
+      // causal: key k is hidden from query q where k - shift > q; `first` is
+      // that of this wave's first key against the tile's first query
+      const int64_t first = k0 - shift - (int64_t)t * kGT;
+      step(slot * kPair, slot == 0 ? 2 : slot - 1, (int)max(min(first, (int64_t)2 * kGT), (int64_t)-2 * kGT));
+      if (++t == nqt) t = t0;
+      slot = slot == 2 ? 0 : slot + 1;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  // lane: key 16 i + c16, d = 16 db + 4 kg .. + 3; keys behind the sequence: 0
+#pragma unroll
+  for (int i = 0; i < KB; ++i) {
+    const int64_t ki = k0 + 16 * i + c16;
+    if (ki >= a.nk) continue;
+    const bool live = ki < nkb;
+    if (a.splits > 1) {
+      const int64_t all_keys = a.batch * a.kv_heads * a.nk * D;
+      float* o = a.part + (int64_t)part * 2 * all_keys + (bh * a.nk + ki) * D + 4 * kg;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        *(f32x4*)(o + 16 * d) = live ? dk[d][i] * a.scale : zero;
+        *(f32x4*)(o + all_keys + 16 * d) = live ? dv[d][i] : zero;
+      }
+      continue;
+    }
+    uint16_t* ok = a.dk + b * a.dk_s[0] + ki * a.dk_s[1] + (int64_t)hk * a.dk_s[2] + 4 * kg;
+    uint16_t* ov = a.dv + b * a.dv_s[0] + ki * a.dv_s[1] + (int64_t)hk * a.dv_s[2] + 4 * kg;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const f32x4 x = dk[d][i] * a.scale, y = dv[d][i];
+      const uint2 none = make_uint2(0, 0);
+      *(uint2*)(ok + 16 * d) = live ? make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])) : none;
+      *(uint2*)(ov + 16 * d) = live ? make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])) : none;
+    }
+  }
+}
+
+// dk and dv from their parts, in part order; 8 values a thread.
+template <int D>
+__global__ __launch_bounds__(256) void k_attn_dkv_join(AttnGradArgs a) {
+  const int64_t all = a.batch * a.kv_heads * a.nk * D;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (i >= 2 * all) return;
+  const bool second = i >= all;
+  const int64_t e = second ? i - all : i;
+  float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int p = 0; p < a.splits; ++p) {
+    const float* f = a.part + (int64_t)p * 2 * all + i;
+    const float4 u = *(const float4*)f, v = *(const float4*)(f + 4);
+    s[0] += u.x, s[1] += u.y, s[2] += u.z, s[3] += u.w, s[4] += v.x, s[5] += v.y, s[6] += v.z, s[7] += v.w;
+  }
+  const int64_t row = e / D;  // (b, hk, key)
+  const int64_t bh = row / a.nk, key = row - bh * a.nk;
+  const int64_t b = bh / a.kv_heads, hk = bh - b * a.kv_heads;
+  uint16_t* o = second ? a.dv + b * a.dv_s[0] + key * a.dv_s[1] + hk * a.dv_s[2]
+                       : a.dk + b * a.dk_s[0] + key * a.dk_s[1] + hk * a.dk_s[2];
+  *(uint4*)(o + e % D) = pack8(s);
+}
+
+// -------------------------------------------------------------------- host
+static int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+// Parts of a key block's query steps: as many as bring the launch to two
+// workgroups a CU, each of at least four steps.
+static int dkv_splits(int64_t batch, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads) {
+  const int64_t wgs = batch * kv_heads * ((nk + 255) / 256);
+  const int64_t steps = (nq + kGT - 1) / kGT * (heads / kv_heads);
+  const int64_t want = 2 * (int64_t)cu_count() / wgs;
+  return (int)max((int64_t)1, min(min(want, steps / 4), (int64_t)16));
+}
+
+static bool grad_strides(const void* p, const int64_t* s, int64_t tokens) {
+  if (!p || !aligned(p, 16)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (s[i] % 8) return false;
+  return tokens <= 1 || (s[1] >= 0 && s[1] < (1 << 24));  // a tile's offsets are 32-bit
+}
+
+static int grad_shape(AttnGradArgs& a, int64_t batch, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads,
+                      int64_t head_dim, float scale, int causal, const int32_t* k_lens) {
+  if (head_dim != 64 && head_dim != 128) return unsupported("head_dim %lld", (long long)head_dim);
+  if (batch < 1 || nq < 1 || nk < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads)
+    return fail("shape (%lld, %lld, %lld, %lld, %lld)", (long long)batch, (long long)nq, (long long)nk,
+                (long long)heads, (long long)kv_heads);
+  if (nq > (1 << 30) || nk > (1 << 30) || heads > (1 << 20) || batch > (1 << 20))
+    return unsupported("shape (%lld, %lld, %lld, %lld)", (long long)batch, (long long)nq, (long long)nk, (long long)heads);
+  if (batch * heads * ((nq + 31) / 32) > INT32_MAX || batch * kv_heads * ((nk + 31) / 32) > INT32_MAX / 16)
+    return unsupported("more than 2^31 workgroups");
+  if ((nq + kGT - 1) / kGT * (heads / kv_heads) > INT32_MAX / 64) return unsupported("too many queries per key head");
+  if (!(scale > 0.0f) || scale > 1e30f) return fail("softmax scale");
+  if (!aligned(k_lens, 4)) return fail("k_lens alignment");
+  a.batch = batch, a.nq = nq, a.nk = nk;
+  a.heads = (int)heads, a.kv_heads = (int)kv_heads, a.group = (int)(heads / kv_heads);
+  a.scale = scale, a.scale_log2 = scale * kLog2e;
+  a.causal = causal ? 1 : 0;
+  a.k_lens = k_lens;
+  return OGA_OK;
+}
+
+template <int D, int W>
+static void lse_launch(AttnGradArgs& a, hipStream_t s) {
+  a.blocks = (int)((a.nq + 32 * W - 1) / (32 * W));
+  const dim3 grid((unsigned)(a.batch * a.heads * a.blocks)), block(64 * W);
+  if (a.causal)
+    k_attn_lse<D, W, true><<<grid, block, 0, s>>>(a);
+  else
+    k_attn_lse<D, W, false><<<grid, block, 0, s>>>(a);
+}
+
+template <int D>
+static void bwd_launch(AttnGradArgs& a, hipStream_t s) {
+  const int64_t nqp = (a.nq + kGT - 1) / kGT * kGT;
+  const int per = 256 / (D / 8);
+  k_attn_delta<D><<<dim3((unsigned)((a.batch * nqp * a.heads + per - 1) / per)), dim3(256), 0, s>>>(a);
+  const dim3 block(64 * kGW);
+  a.blocks = (int)((a.nq + 32 * kGW - 1) / (32 * kGW));
+  const dim3 gq((unsigned)(a.batch * a.heads * a.blocks));
+  if (a.causal)
+    k_attn_dq<D, true><<<gq, block, 0, s>>>(a);
+  else
+    k_attn_dq<D, false><<<gq, block, 0, s>>>(a);
+  a.blocks = (int)((a.nk + DkvShape<D>::kKeys - 1) / DkvShape<D>::kKeys);
+  const dim3 gk((unsigned)(a.batch * a.kv_heads * a.blocks * a.splits)), bk(64 * DkvShape<D>::kW);
+  if (a.causal)
+    k_attn_dkv<D, true><<<gk, bk, 0, s>>>(a);
+  else
+    k_attn_dkv<D, false><<<gk, bk, 0, s>>>(a);
+  if (a.splits > 1) {
+    const int64_t n = 2 * a.batch * a.kv_heads * a.nk * D / 8;
+    k_attn_dkv_join<D><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s>>>(a);
+  }
+}
+
+static void gset3(int64_t* d, const int64_t* s) { d[0] = s[0], d[1] = s[1], d[2] = s[2]; }
+
+}  // namespace oga
+
+using namespace oga;
+
+extern "C" int oga_attention_lse(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
+                                 const void* v, const int64_t v_strides[3], void* o, const int64_t o_strides[3],
+                                 float* lse, int64_t batch, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads,
+                                 int64_t head_dim, float softmax_scale, int causal, const int32_t* k_lens,
+                                 void* stream) {
+  AttnGradArgs a = {};
+  if (int rc = grad_shape(a, batch, nq, nk, heads, kv_heads, head_dim, softmax_scale, causal, k_lens)) return rc;
+  if (!grad_strides(q, q_strides, nq) || !grad_strides(k, k_strides, nk) || !grad_strides(v, v_strides, nk) ||
+      !grad_strides(o, o_strides, nq) || !lse || !aligned(lse, 4))
+    return fail("operand layout");
+  a.q = (const uint16_t*)q, a.k = (const uint16_t*)k, a.v = (const uint16_t*)v, a.o = (uint16_t*)o, a.lse = lse;
+  gset3(a.q_s, q_strides), gset3(a.k_s, k_strides), gset3(a.v_s, v_strides), gset3(a.o_s, o_strides);
+  const hipStream_t s = (hipStream_t)stream;
+  if (head_dim == 128)
+    nq > 64 ? lse_launch<128, 8>(a, s) : lse_launch<128, 2>(a, s);
+  else
+    nq > 64 ? lse_launch<64, 8>(a, s) : lse_launch<64, 2>(a, s);
+  return launch_status();
+}
+
+extern "C" int64_t oga_attention_bwd_workspace_bytes(int64_t batch, int64_t nq, int64_t nk, int64_t heads,
+                                                     int64_t kv_heads, int64_t head_dim) {
+  if (batch < 1 || nq < 1 || nk < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads) return 0;
+  const int64_t ld = align256(batch * heads * ((nq + kGT - 1) / kGT) * 128 * 4);
+  const int splits = dkv_splits(batch, nq, nk, heads, kv_heads);
+  return ld + (splits > 1 ? splits * 2 * batch * kv_heads * nk * head_dim * 4 : 0);
+}
+
+extern "C" int oga_attention_bwd(const void* dout, const int64_t do_strides[3], const void* q,
+                                 const int64_t q_strides[3], const void* k, const int64_t k_strides[3], const void* v,
+                                 const int64_t v_strides[3], const void* out, const int64_t o_strides[3],
+                                 const float* lse, void* dq, const int64_t dq_strides[3], void* dk,
+                                 const int64_t dk_strides[3], void* dv, const int64_t dv_strides[3], int64_t batch,
+                                 int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                 float softmax_scale, int causal, const int32_t* k_lens, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  AttnGradArgs a = {};
+  if (int rc = grad_shape(a, batch, nq, nk, heads, kv_heads, head_dim, softmax_scale, causal, k_lens)) return rc;
+  if (!grad_strides(dout, do_strides, nq) || !grad_strides(q, q_strides, nq) || !grad_strides(k, k_strides, nk) ||
+      !grad_strides(v, v_strides, nk) || !grad_strides(out, o_strides, nq) || !grad_strides(dq, dq_strides, nq) ||
+      !grad_strides(dk, dk_strides, nk) || !grad_strides(dv, dv_strides, nk) || !lse || !aligned(lse, 4))
+    return fail("operand layout");
+  const int64_t need = oga_attention_bwd_workspace_bytes(batch, nq, nk, heads, kv_heads, head_dim);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
+    return fail("workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  a.dout = (const uint16_t*)dout, a.q = (const uint16_t*)q, a.k = (const uint16_t*)k, a.v = (const uint16_t*)v;
+  a.out = (const uint16_t*)out, a.lse = const_cast<float*>(lse);
+  a.dq = (uint16_t*)dq, a.dk = (uint16_t*)dk, a.dv = (uint16_t*)dv;
+  gset3(a.do_s, do_strides), gset3(a.q_s, q_strides), gset3(a.k_s, k_strides), gset3(a.v_s, v_strides);
+  gset3(a.o_s, o_strides), gset3(a.dq_s, dq_strides), gset3(a.dk_s, dk_strides), gset3(a.dv_s, dv_strides);
+  a.ld = (float*)workspace;
+  a.splits = dkv_splits(batch, nq, nk, heads, kv_heads);
+  a.part = (float*)((char*)workspace + align256(batch * heads * ((nq + kGT - 1) / kGT) * 128 * 4));
+  const hipStream_t s = (hipStream_t)stream;
+  if (head_dim == 128)
+    bwd_launch<128>(a, s);
+  else
+    bwd_launch<64>(a, s);
+  return launch_status();
+}

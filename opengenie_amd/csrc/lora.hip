@@ -1,0 +1,645 @@
+// Low-rank adapters of many requests beside a shared projection, and their
+// backward pass.
+//
+// Rows (tokens) are divided into segments, each with an adapter l (or none):
+//   y' = y + s_l B_l (A_l x)          A_l [r, K], B_l [N, r]
+//   dx = A_l^T dlow,  dlow = s_l B_l^T dy
+//   dA_l = sum_rows dlow x^T,  dB_l = sum_rows dy low^T,  low = s_l A_l x.
+// r is small, so every product is bound by moving x, y and dy once:
+//  * k_lora_shrink: low (or dlow) [rows, r], float32, from the long rows. The
+//    waves of a workgroup divide the long axis and add up in LDS.
+//  * k_lora_expand: the [rows, N] (or [rows, K]) result from low, added to y.
+//  * k_lora_wgrad: dA and dB, one workgroup per adapter, 512 columns and part
+//    of the adapter's rows; k_lora_join adds the parts in order.
+// The sums low and dlow stay float32 in memory and enter the matrix products
+// as two 16-bit halves (v = hi + lo), so only results are rounded.
+//
+// The segments are device data (no host synchronisation): a row tile of BM
+// rows is paired with each segment it meets. With the bounds b_0 = 0,
+// b_1 .. b_{S+1} (the starts) and b_{S+2} = T of S + 2 segments (the first and
+// last without an adapter), pair number floor(b_s / BM) + s + j is tile
+// floor(b_s / BM) + j of segment s: unique, since each next segment begins in
+// the last tile of the one before or later, and below ceil(T / BM) + S + 2.
+#include "common.h"
+#include "host.h"
+
+namespace oga {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// C[16 x 16] += A[16 x 32] B[32 x 16]: lane l has row (A) or column (B) l % 16
+// at k = 8 (l / 16) .. +7, and of C column l % 16, rows 4 (l / 16) .. +3.
+template <int XDT>
+OGA_DEVICE f32x4 mfma16(const uint4& a, const uint4& b, const f32x4& c) {
+  if constexpr (XDT == OGA_DT_F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+}
+
+template <int XDT>
+OGA_DEVICE uint32_t pack2x(float a, float b) {
+  return XDT == OGA_DT_F16 ? pack_f16(a, b) : pack_bf16(a, b);
+}
+template <int XDT>
+OGA_DEVICE uint4 pack8x(const float* f) {
+  return make_uint4(pack2x<XDT>(f[0], f[1]), pack2x<XDT>(f[2], f[3]), pack2x<XDT>(f[4], f[5]),
+                    pack2x<XDT>(f[6], f[7]));
+}
+// The two 16-bit halves of 8 floats.
+template <int XDT>
+OGA_DEVICE void split8x(const float* f, uint4& hi, uint4& lo) {
+  hi = pack8x<XDT>(f);
+  float h[8], d[8];
+  unpack8x<XDT>(hi, h);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) d[i] = f[i] - h[i];
+  lo = pack8x<XDT>(d);
+}
+
+struct Segments {
+  const int32_t* starts;  // [count + 1]
+  const int32_t* ids;     // [count]
+  int count;
+  int adapters;
+  int64_t rows;
+};
+
+// Bounds of segment s of count + 2 (see above), inside [0, rows] whatever
+// the starts say.
+OGA_DEVICE int64_t seg_bound(const Segments& g, int s) {
+  if (s <= 0) return 0;
+  if (s > g.count + 1) return g.rows;
+  return min(max((int64_t)g.starts[s - 1], (int64_t)0), g.rows);
+}
+
+struct Pair {
+  int64_t lo, hi, tile0;  // rows lo .. hi - 1 (none: hi <= lo) of the tile that begins at row tile0
+  int adapter;            // -1: none
+};
+
+// Pair number p for tiles of BM rows. Lanes test 64 segments at a time.
+template <int BM>
+OGA_DEVICE Pair seg_pair(const Segments& g, int64_t p, int lane) {
+  const int all = g.count + 2;
+  int seg = 0;
+  int64_t b0 = 0;
+  for (int s0 = 0; s0 < all; s0 += 64) {
+    const int s = s0 + lane;
+    const int64_t b = s < all ? seg_bound(g, s) : 0;
+    const unsigned long long m = __ballot(s < all && b / BM + s <= p);
+    if (!m) break;
+    const int top = 63 - __builtin_clzll(m);
+    seg = s0 + top;
+    b0 = (int64_t)__builtin_amdgcn_readlane((int)b, top);  // rows stay below 2^31
+    if (top < 63) break;
+  }
+  const int64_t b1 = seg_bound(g, seg + 1);
+  Pair r;
+  r.tile0 = (p - seg) * BM;  // floor(b0 / BM) + j tiles down
+  r.lo = max(b0, r.tile0);
+  r.hi = min(b1, r.tile0 + BM);
+  const int id = seg >= 1 && seg <= g.count ? g.ids[seg - 1] : -1;
+  r.adapter = id >= 0 && id < g.adapters ? id : -1;
+  return r;
+}
+
+static int64_t seg_pairs(int64_t rows, int64_t count, int bm) { return (rows + bm - 1) / bm + count + 2; }
+
+// ------------------------------------------------------------------ shrink
+struct ShrinkArgs {
+  Segments g;
+  const void* x;  // [rows, k], row stride xs
+  int64_t xs;
+  const void* w;  // [adapters, rank, k]
+  const float* scale;
+  float* low;     // [rows, rank]
+  int64_t k;
+  int rank;
+};
+
+constexpr int kShrinkWaves = 8;
+
+// 16 TB rows x 16 RB ranks per workgroup; wave w takes an eighth of the long
+// axis. The fragments come straight from memory (each row's 64-byte pieces of
+// consecutive steps share a line).
+template <int XDT, int RB, int TB>
+__global__ __launch_bounds__(64 * kShrinkWaves) void k_lora_shrink(ShrinkArgs a) {
+  __shared__ f32x4 red[kShrinkWaves][TB * RB][64];
+  const int lane = threadIdx.x & 63;
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const Pair p = seg_pair<16 * TB>(a.g, blockIdx.x, lane);
+  if (p.adapter < 0 || p.hi <= p.lo) return;  // (uniform over the workgroup)
+  const int c = lane & 15, kg = 8 * (lane >> 4);
+  const uint16_t* xr[TB];
+#pragma unroll
+  for (int t = 0; t < TB; ++t)
+    xr[t] = (const uint16_t*)a.x + min(max(p.tile0 + 16 * t + c, p.lo), p.hi - 1) * a.xs;
+  const uint16_t* wr[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r)
+    wr[r] = (const uint16_t*)a.w + ((int64_t)p.adapter * a.rank + min(16 * r + c, a.rank - 1)) * a.k;
+  f32x4 acc[TB][RB];
+#pragma unroll
+  for (int t = 0; t < TB; ++t)
+#pragma unroll
+    for (int r = 0; r < RB; ++r) acc[t][r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const int64_t steps = (a.k + 31) / 32, whole = a.k / 32;
+  const int64_t s0 = steps * wv / kShrinkWaves, s1 = steps * (wv + 1) / kShrinkWaves;
+  auto step = [&](int64_t k0, bool in) {
+    uint4 xf[TB], wf[RB];
+    const uint4 none = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int t = 0; t < TB; ++t) xf[t] = in ? *(const uint4*)(xr[t] + k0) : none;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) wf[r] = in ? *(const uint4*)(wr[r] + k0) : none;
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int t = 0; t < TB; ++t) acc[t][r] = mfma16<XDT>(wf[r], xf[t], acc[t][r]);
+  };
+#pragma unroll 4
+  for (int64_t s = s0; s < min(s1, whole); ++s) step(32 * s + kg, true);
+  if (s1 > whole && s1 > s0) step(32 * whole + kg, 32 * whole + kg < a.k);
+#pragma unroll
+  for (int t = 0; t < TB; ++t)
+#pragma unroll
+    for (int r = 0; r < RB; ++r) red[wv][t * RB + r][lane] = acc[t][r];
+  __syncthreads();
+  const float scale = a.scale ? a.scale[p.adapter] : 1.0f;
+  for (int o = wv; o < TB * RB; o += kShrinkWaves) {
+    f32x4 v = red[0][o][lane];
+#pragma unroll
+    for (int w = 1; w < kShrinkWaves; ++w) v += red[w][o][lane];
+    const int64_t row = p.tile0 + 16 * (o / RB) + c;
+    const int rank = 16 * (o % RB) + 4 * (lane >> 4);
+    if (row >= p.lo && row < p.hi && rank < a.rank) *(f32x4*)(a.low + row * a.rank + rank) = v * scale;
+  }
+}
+
+// ------------------------------------------------------------------ expand
+struct ExpandArgs {
+  Segments g;
+  const float* low;  // [rows, rank]
+  const void* w;     // [adapters, n, rank]
+  const void* y;     // [rows, n] or null (zero)
+  void* out;         // [rows, n]; may be y
+  int64_t ys, os;    // row strides
+  int64_t n;
+  int rank;
+  int groups;        // 32-column groups per wave
+};
+
+constexpr int kExpandWaves = 4;
+
+// 16 TB rows x 32 groups columns per wave. The features of the two MFMA row
+// blocks of a group interleave by fours (block b's row 4g + i is column
+// 8g + 4b + i), so a lane ends with 8 consecutive columns of its row.
+template <int XDT, int KS, int TB>
+__global__ __launch_bounds__(64 * kExpandWaves) void k_lora_expand(ExpandArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const Pair p = seg_pair<16 * TB>(a.g, blockIdx.x, lane);
+  if (p.hi <= p.lo) return;
+  const int c = lane & 15, kg = 8 * (lane >> 4);
+  const int64_t f_begin = ((int64_t)blockIdx.y * kExpandWaves + wv) * 32 * a.groups;
+  const int64_t f_end = min(f_begin + 32 * a.groups, a.n);
+  if (f_begin >= f_end) return;
+  if (p.adapter < 0) {  // rows without an adapter keep y (dx: zero)
+    if (a.y == a.out) return;
+    for (int64_t f = f_begin + kg; f < f_end; f += 32)
+#pragma unroll
+      for (int t = 0; t < TB; ++t) {
+        const int64_t row = p.tile0 + 16 * t + c;
+        if (row < p.lo || row >= p.hi) continue;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (a.y) v = *(const uint4*)((const uint16_t*)a.y + row * a.ys + f);
+        *(uint4*)((uint16_t*)a.out + row * a.os + f) = v;
+      }
+    return;
+  }
+  uint4 hi[TB][KS], lo[TB][KS];
+#pragma unroll
+  for (int t = 0; t < TB; ++t) {
+    const float* l = a.low + min(max(p.tile0 + 16 * t + c, p.lo), p.hi - 1) * a.rank;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (32 * s + kg < a.rank) {
+        const float4 u = *(const float4*)(l + 32 * s + kg), v = *(const float4*)(l + 32 * s + kg + 4);
+        f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = v.x, f[5] = v.y, f[6] = v.z, f[7] = v.w;
+      }
+      split8x<XDT>(f, hi[t][s], lo[t][s]);
+    }
+  }
+  const uint16_t* w = (const uint16_t*)a.w + (int64_t)p.adapter * a.n * a.rank;
+  for (int64_t f0 = f_begin; f0 < f_end; f0 += 32) {
+    const int64_t f = f0 + kg;  // this lane's 8 columns
+    uint4 yv[TB];
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+      const int64_t row = min(max(p.tile0 + 16 * t + c, p.lo), p.hi - 1);
+      yv[t] = a.y && f < a.n ? *(const uint4*)((const uint16_t*)a.y + row * a.ys + f) : make_uint4(0, 0, 0, 0);
+    }
+    f32x4 acc[2][TB];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int64_t feat = min(f0 + 8 * (c >> 2) + 4 * b + (c & 3), a.n - 1);
+      uint4 wf[KS];
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        wf[s] = 32 * s + kg < a.rank ? *(const uint4*)(w + feat * a.rank + 32 * s + kg) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < TB; ++t) {
+        acc[b][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          acc[b][t] = mfma16<XDT>(wf[s], lo[t][s], acc[b][t]);
+          acc[b][t] = mfma16<XDT>(wf[s], hi[t][s], acc[b][t]);
+        }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+      const int64_t row = p.tile0 + 16 * t + c;
+      float v[8];
+      unpack8x<XDT>(yv[t], v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = a.y ? v[i] + acc[i >> 2][t][i & 3] : acc[i >> 2][t][i & 3];
+      if (row >= p.lo && row < p.hi && f < a.n) *(uint4*)((uint16_t*)a.out + row * a.os + f) = pack8x<XDT>(v);
+    }
+  }
+}
+
+// -------------------------------------------------------- 16-bit transpose
+// dst[l][c][r] = src[l][r][c] for the two weights (A and B) of one call.
+struct TransposeArgs {
+  const uint16_t* src[2];
+  uint16_t* dst[2];
+  int64_t rows[2], cols[2];
+  int64_t blocks0;     // workgroups of the first
+  int64_t tiles[2];    // 32 x 32 tiles per adapter
+  int64_t col_tiles[2];
+};
+__global__ __launch_bounds__(256) void k_lora_transpose(TransposeArgs a) {
+  __shared__ uint16_t tile[32][33];
+  const int i = (int64_t)blockIdx.x >= a.blocks0;
+  const int64_t u = (int64_t)blockIdx.x - (i ? a.blocks0 : 0);
+  const int64_t rows = i ? a.rows[1] : a.rows[0], cols = i ? a.cols[1] : a.cols[0];
+  const int64_t tiles = i ? a.tiles[1] : a.tiles[0], ct = i ? a.col_tiles[1] : a.col_tiles[0];
+  const int64_t l = u / tiles, t = u - l * tiles;
+  const int64_t r0 = t / ct * 32, c0 = t % ct * 32;
+  const uint16_t* src = (i ? a.src[1] : a.src[0]) + l * rows * cols;
+  uint16_t* dst = (i ? a.dst[1] : a.dst[0]) + l * rows * cols;
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+#pragma unroll
+  for (int j = 0; j < 32; j += 8)
+    if (r0 + y + j < rows && c0 + x < cols) tile[y + j][x] = src[(r0 + y + j) * cols + c0 + x];
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 32; j += 8)
+    if (c0 + y + j < cols && r0 + x < rows) dst[(c0 + y + j) * rows + r0 + x] = tile[x][y + j];
+}
+
+// ------------------------------------------------------- weight gradients
+struct WgradSide {
+  const void* x;     // [rows, c]: x for dA, dy for dB
+  int64_t xs;
+  const float* u;    // [rows, rank]: dlow for dA, low for dB
+  int64_t c;
+  float* part;       // [adapters][splits][rank][c]
+  int col_tiles;     // of 512 columns
+};
+struct WgradArgs {
+  Segments g;
+  WgradSide side[2];
+  int rank, splits;
+};
+
+constexpr int kWgradRows = 128;  // rows of one pass over LDS
+constexpr int kWgradPad = kWgradRows + 8;
+
+// One adapter, 4 x 128 columns, ranks 16 RB z .. , every splits-th 128-row
+// tile of the adapter's segments. A lane loads 8 rows x 8 columns (16 lanes
+// cover 256 bytes of a row) and regroups them by column with one v_perm per
+// dword: column c of lanes is an MFMA operand whose k runs over rows.
+template <int XDT, int RB>
+__global__ __launch_bounds__(256) void k_lora_wgrad(WgradArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t uh[16 * RB * kWgradPad], ul[16 * RB * kWgradPad];
+  const int lane = threadIdx.x & 63;
+  const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const bool second = (int)blockIdx.x >= a.side[0].col_tiles;
+  const WgradSide& sd = second ? a.side[1] : a.side[0];
+  const int ct = (int)blockIdx.x - (second ? a.side[0].col_tiles : 0);
+  const int adapter = blockIdx.y / a.splits, split = blockIdx.y % a.splits;
+  const int r0 = 16 * RB * blockIdx.z;
+  const int c = lane & 15, g8 = 8 * (lane >> 4);
+  const int64_t col = (int64_t)ct * 512 + wv * 128 + 8 * c;
+  const int64_t colc = min(col, sd.c - 8);
+  f32x4 acc[8][RB];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int r = 0; r < RB; ++r) acc[j][r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  int64_t seen = 0;  // tiles of this adapter so far
+  auto tile = [&](int64_t lo, int64_t hi) {
+    __syncthreads();  // the last tile's reads are done
+    const int n4 = 4 * RB;  // float4 per row
+    for (int i = threadIdx.x; i < kWgradRows * n4; i += 256) {
+      const int row = i / n4, q = i % n4;
+      float4 v = make_float4(0, 0, 0, 0);
+      if (lo + row < hi && r0 + 4 * q < a.rank) v = *(const float4*)(sd.u + (lo + row) * a.rank + r0 + 4 * q);
+      const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t h = pack2x<XDT>(f[e], 0.0f) & 0xFFFFu;
+        uh[(4 * q + e) * kWgradPad + row] = (uint16_t)h;
+        ul[(4 * q + e) * kWgradPad + row] = (uint16_t)(pack2x<XDT>(f[e] - x16_bits<XDT>(h), 0.0f) & 0xFFFFu);
+      }
+    }
+    __syncthreads();
+    const int steps = (int)((min(hi - lo, (int64_t)kWgradRows) + 31) / 32);
+    for (int st = 0; st < steps; ++st) {
+      const int64_t row = lo + 32 * st + g8;
+      uint4 xv[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        xv[j] = make_uint4(0, 0, 0, 0);  // rows of others may hold anything
+        if (row + j < hi) xv[j] = *(const uint4*)((const uint16_t*)sd.x + (row + j) * sd.xs + colc);
+      }
+      uint4 fh[RB], fl[RB];
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const int at = (16 * r + c) * kWgradPad + 32 * st + g8;
+        fh[r] = *(const uint4*)(uh + at);
+        fl[r] = *(const uint4*)(ul + at);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+        auto word = [&](const uint4& v) { return (j >> 1) == 0 ? v.x : (j >> 1) == 1 ? v.y : (j >> 1) == 2 ? v.z : v.w; };
+        const uint4 xf = make_uint4(__builtin_amdgcn_perm(word(xv[1]), word(xv[0]), sel),
+                                    __builtin_amdgcn_perm(word(xv[3]), word(xv[2]), sel),
+                                    __builtin_amdgcn_perm(word(xv[5]), word(xv[4]), sel),
+                                    __builtin_amdgcn_perm(word(xv[7]), word(xv[6]), sel));
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          acc[j][r] = mfma16<XDT>(fl[r], xf, acc[j][r]);
+          acc[j][r] = mfma16<XDT>(fh[r], xf, acc[j][r]);
+        }
+      }
+    }
+  };
+  for (int s0 = 0; s0 < a.g.count; s0 += 64) {
+    const int s = s0 + lane;
+    const bool mine = s < a.g.count && a.g.ids[s] == adapter;
+    const int64_t b0 = mine ? seg_bound(a.g, s + 1) : 0, b1 = mine ? seg_bound(a.g, s + 2) : 0;
+    unsigned long long m = __ballot(mine && b0 < b1);
+    while (m) {
+      const int l = __builtin_ctzll(m);
+      m &= m - 1;
+      const int64_t lo = __builtin_amdgcn_readlane((int)b0, l), hi = __builtin_amdgcn_readlane((int)b1, l);
+      for (int64_t t = lo; t < hi; t += kWgradRows, ++seen)
+        if (seen % a.splits == split) tile(t, hi);
+    }
+  }
+  if (col >= sd.c) return;
+  float* part = sd.part + ((int64_t)adapter * a.splits + split) * a.rank * sd.c;
+#pragma unroll
+  for (int r = 0; r < RB; ++r)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int rank = r0 + 16 * r + 4 * (lane >> 4) + i;
+      if (rank >= a.rank) continue;
+      float* o = part + (int64_t)rank * sd.c + col;
+      *(float4*)o = make_float4(acc[0][r][i], acc[1][r][i], acc[2][r][i], acc[3][r][i]);
+      *(float4*)(o + 4) = make_float4(acc[4][r][i], acc[5][r][i], acc[6][r][i], acc[7][r][i]);
+    }
+}
+
+struct JoinArgs {
+  const float* part[2];  // [adapters][splits][rank][c]
+  uint16_t* out[2];      // dA [adapters][rank][k], dB [adapters][n][rank]
+  int64_t c[2];
+  int64_t blocks0;       // workgroups of the first
+  int64_t adapters;
+  int rank, splits;
+};
+// Four columns of one rank (dA) or one column's four ranks (dB) a thread.
+template <int XDT>
+__global__ __launch_bounds__(256) void k_lora_join(JoinArgs a) {
+  const bool second = (int64_t)blockIdx.x >= a.blocks0;
+  const int64_t c = second ? a.c[1] : a.c[0];
+  const int64_t i = ((int64_t)blockIdx.x - (second ? a.blocks0 : 0)) * 256 + threadIdx.x;
+  const int64_t per = a.rank * c / 4;
+  if (i >= a.adapters * per) return;
+  const int64_t l = i / per, e = i - l * per;
+  const float* part = (second ? a.part[1] : a.part[0]) + l * a.splits * a.rank * c;
+  float v[4] = {0, 0, 0, 0};
+  if (!second) {
+    for (int s = 0; s < a.splits; ++s) {
+      const float4 u = *(const float4*)(part + (int64_t)s * a.rank * c + 4 * e);
+      v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w;
+    }
+    *(uint2*)(a.out[0] + l * a.rank * c + 4 * e) = make_uint2(pack2x<XDT>(v[0], v[1]), pack2x<XDT>(v[2], v[3]));
+  } else {
+    const int64_t q = e / c, col = e - q * c;  // ranks 4q .. 4q + 3: a wave reads consecutive columns
+    for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] += part[((int64_t)s * a.rank + 4 * q + r) * c + col];
+    *(uint2*)(a.out[1] + (l * c + col) * a.rank + 4 * q) = make_uint2(pack2x<XDT>(v[0], v[1]), pack2x<XDT>(v[2], v[3]));
+  }
+}
+
+// -------------------------------------------------------------------- host
+// Rows of a tile: 16 where segments are short (a step's single tokens), more
+// where they are long and each fragment of the weights serves more rows.
+static bool long_segments(const Segments& g) { return g.rows >= 64 * (int64_t)g.count; }
+
+template <int XDT, int RB>
+static void shrink_launch(const ShrinkArgs& a, hipStream_t s) {
+  constexpr int TB = RB >= 8 ? 1 : 2;
+  if (long_segments(a.g))
+    k_lora_shrink<XDT, RB, TB><<<dim3((unsigned)seg_pairs(a.g.rows, a.g.count, 16 * TB)), dim3(64 * kShrinkWaves), 0, s>>>(a);
+  else
+    k_lora_shrink<XDT, RB, 1><<<dim3((unsigned)seg_pairs(a.g.rows, a.g.count, 16)), dim3(64 * kShrinkWaves), 0, s>>>(a);
+}
+template <int XDT>
+static void shrink(const ShrinkArgs& a, hipStream_t s) {
+  if (a.rank <= 16)
+    shrink_launch<XDT, 1>(a, s);
+  else if (a.rank <= 32)
+    shrink_launch<XDT, 2>(a, s);
+  else if (a.rank <= 64)
+    shrink_launch<XDT, 4>(a, s);
+  else
+    shrink_launch<XDT, 8>(a, s);
+}
+
+template <int XDT, int KS>
+static void expand_launch(ExpandArgs a, hipStream_t s) {
+  constexpr int TB = KS >= 4 ? 2 : 4;
+  const bool wide = long_segments(a.g);
+  a.groups = wide ? 4 : 1;
+  const unsigned gy = (unsigned)((a.n + 32 * a.groups * kExpandWaves - 1) / (32 * a.groups * kExpandWaves));
+  if (wide)
+    k_lora_expand<XDT, KS, TB><<<dim3((unsigned)seg_pairs(a.g.rows, a.g.count, 16 * TB), gy), dim3(64 * kExpandWaves), 0, s>>>(a);
+  else
+    k_lora_expand<XDT, KS, 1><<<dim3((unsigned)seg_pairs(a.g.rows, a.g.count, 16), gy), dim3(64 * kExpandWaves), 0, s>>>(a);
+}
+template <int XDT>
+static void expand(const ExpandArgs& a, hipStream_t s) {
+  if (a.rank <= 32)
+    expand_launch<XDT, 1>(a, s);
+  else if (a.rank <= 64)
+    expand_launch<XDT, 2>(a, s);
+  else
+    expand_launch<XDT, 4>(a, s);
+}
+
+static int wgrad_rank_blocks(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : 4; }
+
+// Parts of each adapter's rows: enough workgroups for two a CU, but no more
+// than tiles of 128 rows an adapter has on average.
+static int wgrad_splits(int64_t rows, int64_t adapters, int64_t k, int64_t n, int64_t rank) {
+  const int64_t rz = (rank + 16 * wgrad_rank_blocks((int)rank) - 1) / (16 * wgrad_rank_blocks((int)rank));
+  const int64_t wgs = ((k + 511) / 512 + (n + 511) / 512) * adapters * rz;
+  const int64_t want = (2 * (int64_t)cu_count() + wgs - 1) / wgs;
+  const int64_t tiles = (rows + kWgradRows * adapters - 1) / (kWgradRows * adapters);
+  return (int)max((int64_t)1, min(min(want, tiles), (int64_t)32));
+}
+
+template <int XDT>
+static void wgrad(const WgradArgs& a, hipStream_t s) {
+  const int rb = wgrad_rank_blocks(a.rank);
+  const dim3 grid((unsigned)(a.side[0].col_tiles + a.side[1].col_tiles), (unsigned)(a.g.adapters * a.splits),
+                  (unsigned)((a.rank + 16 * rb - 1) / (16 * rb)));
+  if (rb == 1)
+    k_lora_wgrad<XDT, 1><<<grid, dim3(256), 0, s>>>(a);
+  else if (rb == 2)
+    k_lora_wgrad<XDT, 2><<<grid, dim3(256), 0, s>>>(a);
+  else
+    k_lora_wgrad<XDT, 4><<<grid, dim3(256), 0, s>>>(a);
+}
+
+static int lora_shape(int x_dtype, int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters,
+                      int64_t segments, const void* starts, const void* ids) {
+  if (x_dtype != OGA_DT_BF16 && x_dtype != OGA_DT_F16) return fail("x dtype code %d", x_dtype);
+  if (rows < 1 || k < 8 || n < 8 || k % 8 || n % 8) return fail("shape rows %lld, k %lld, n %lld", (long long)rows,
+                                                                (long long)k, (long long)n);
+  if (rank < 8 || rank > 128 || rank % 8) return unsupported("rank %lld", (long long)rank);
+  if (adapters < 1 || segments < 1 || adapters > 2000 || segments > (1 << 20))
+    return fail("%lld adapters, %lld segments", (long long)adapters, (long long)segments);
+  if (rows > (1 << 30) || k > (1 << 22) || n > (1 << 22))
+    return unsupported("rows %lld, k %lld, n %lld", (long long)rows, (long long)k, (long long)n);
+  if (!starts || !ids || !aligned(starts, 4) || !aligned(ids, 4)) return fail("segments");
+  return OGA_OK;
+}
+static bool rows_ok(const void* p, int64_t stride) { return p && aligned(p, 16) && stride % 8 == 0; }
+
+static int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+// Layout of the backward workspace: dlow, A^T, B^T, the partial dA and dB.
+struct LoraBwdSpace {
+  int64_t dlow, at, bt, pa, pb, total;
+  int splits;
+};
+static LoraBwdSpace lora_bwd_space(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
+  LoraBwdSpace w;
+  w.splits = wgrad_splits(rows, adapters, k, n, rank);
+  w.dlow = 0;
+  w.at = w.dlow + align256(rows * rank * 4);
+  w.bt = w.at + align256(adapters * rank * k * 2);
+  w.pa = w.bt + align256(adapters * rank * n * 2);
+  w.pb = w.pa + align256(adapters * w.splits * rank * k * 4);
+  w.total = w.pb + align256(adapters * w.splits * rank * n * 4);
+  return w;
+}
+
+}  // namespace oga
+
+using namespace oga;
+
+extern "C" int oga_lora_add(int x_dtype, const void* y, int64_t y_stride, const void* x, int64_t x_stride,
+                            const void* a, const void* b, const float* scale, const int32_t* segment_starts,
+                            const int32_t* segment_adapters, int64_t segments, int64_t adapters, float* low, void* out,
+                            int64_t out_stride, int64_t rows, int64_t k, int64_t n, int64_t rank, void* stream) {
+  if (int rc = lora_shape(x_dtype, rows, k, n, rank, adapters, segments, segment_starts, segment_adapters)) return rc;
+  if (!rows_ok(y, y_stride) || !rows_ok(x, x_stride) || !rows_ok(out, out_stride) || !rows_ok(a, k) ||
+      !rows_ok(b, rank) || !rows_ok(low, 8))
+    return fail("operand alignment");
+  const Segments g = {segment_starts, segment_adapters, (int)segments, (int)adapters, rows};
+  const ShrinkArgs sa = {g, x, x_stride, a, scale, low, k, (int)rank};
+  const ExpandArgs ea = {g, low, b, y, out, y_stride, out_stride, n, (int)rank, 0};
+  const hipStream_t s = (hipStream_t)stream;
+  if (x_dtype == OGA_DT_F16) {
+    shrink<OGA_DT_F16>(sa, s);
+    expand<OGA_DT_F16>(ea, s);
+  } else {
+    shrink<OGA_DT_BF16>(sa, s);
+    expand<OGA_DT_BF16>(ea, s);
+  }
+  return launch_status();
+}
+
+extern "C" int64_t oga_lora_bwd_workspace_bytes(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
+  if (rows < 1 || k < 8 || n < 8 || rank < 8 || rank > 128 || adapters < 1) return 0;
+  return lora_bwd_space(rows, k, n, rank, adapters).total;
+}
+
+extern "C" int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                            const float* low, const void* a, const void* b, const float* scale,
+                            const int32_t* segment_starts, const int32_t* segment_adapters, int64_t segments,
+                            int64_t adapters, void* dx, int64_t dx_stride, void* da, void* db, int64_t rows, int64_t k,
+                            int64_t n, int64_t rank, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (int rc = lora_shape(x_dtype, rows, k, n, rank, adapters, segments, segment_starts, segment_adapters)) return rc;
+  if (!rows_ok(dy, dy_stride) || !rows_ok(x, x_stride) || !rows_ok(dx, dx_stride) || !rows_ok(a, k) ||
+      !rows_ok(b, rank) || !rows_ok(low, 8) || !rows_ok(da, 8) || !rows_ok(db, 8))
+    return fail("operand alignment");
+  const LoraBwdSpace w = lora_bwd_space(rows, k, n, rank, adapters);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < w.total)
+    return fail("workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)w.total);
+  char* const ws = (char*)workspace;
+  float* const dlow = (float*)(ws + w.dlow);
+  const hipStream_t s = (hipStream_t)stream;
+
+  TransposeArgs t = {};
+  t.src[0] = (const uint16_t*)a, t.dst[0] = (uint16_t*)(ws + w.at), t.rows[0] = rank, t.cols[0] = k;
+  t.src[1] = (const uint16_t*)b, t.dst[1] = (uint16_t*)(ws + w.bt), t.rows[1] = n, t.cols[1] = rank;
+  for (int i = 0; i < 2; ++i) {
+    t.col_tiles[i] = (t.cols[i] + 31) / 32;
+    t.tiles[i] = (t.rows[i] + 31) / 32 * t.col_tiles[i];
+  }
+  t.blocks0 = adapters * t.tiles[0];
+  k_lora_transpose<<<dim3((unsigned)(adapters * (t.tiles[0] + t.tiles[1]))), dim3(256), 0, s>>>(t);
+
+  const Segments g = {segment_starts, segment_adapters, (int)segments, (int)adapters, rows};
+  const ShrinkArgs sa = {g, dy, dy_stride, ws + w.bt, scale, dlow, n, (int)rank};
+  const ExpandArgs ea = {g, dlow, ws + w.at, nullptr, dx, 0, dx_stride, k, (int)rank, 0};
+  WgradArgs wa = {};
+  wa.g = g, wa.rank = (int)rank, wa.splits = w.splits;
+  wa.side[0] = {x, x_stride, dlow, k, (float*)(ws + w.pa), (int)((k + 511) / 512)};
+  wa.side[1] = {dy, dy_stride, low, n, (float*)(ws + w.pb), (int)((n + 511) / 512)};
+  JoinArgs j = {};
+  j.part[0] = wa.side[0].part, j.part[1] = wa.side[1].part;
+  j.out[0] = (uint16_t*)da, j.out[1] = (uint16_t*)db;
+  j.c[0] = k, j.c[1] = n;
+  j.adapters = adapters, j.rank = (int)rank, j.splits = w.splits;
+  j.blocks0 = (adapters * rank * k / 4 + 255) / 256;
+  const dim3 jgrid((unsigned)(j.blocks0 + (adapters * rank * n / 4 + 255) / 256));
+  if (x_dtype == OGA_DT_F16) {
+    shrink<OGA_DT_F16>(sa, s);
+    expand<OGA_DT_F16>(ea, s);
+    wgrad<OGA_DT_F16>(wa, s);
+    k_lora_join<OGA_DT_F16><<<jgrid, dim3(256), 0, s>>>(j);
+  } else {
+    shrink<OGA_DT_BF16>(sa, s);
+    expand<OGA_DT_BF16>(ea, s);
+    wgrad<OGA_DT_BF16>(wa, s);
+    k_lora_join<OGA_DT_BF16><<<jgrid, dim3(256), 0, s>>>(j);
+  }
+  return launch_status();
+}

@@ -144,6 +144,15 @@ PyMethodDef kMethods[] = {
     OGA_FN(oga_fp8_dequant_per_head),
     OGA_FN(oga_attention_fp8_workspace_bytes),
     OGA_FN(oga_attention_fp8_ws),
+    OGA_FN(oga_attention_lse),
+    OGA_FN(oga_attention_bwd_workspace_bytes),
+    OGA_FN(oga_attention_bwd),
+    OGA_FN(oga_head_rmsnorm_rope),
+    OGA_FN(oga_head_rmsnorm_rope_bwd_workspace_bytes),
+    OGA_FN(oga_head_rmsnorm_rope_bwd),
+    OGA_FN(oga_lora_add),
+    OGA_FN(oga_lora_bwd_workspace_bytes),
+    OGA_FN(oga_lora_bwd),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", "Entry points of libopengenie_amd.so.", -1, kMethods};

@@ -1,0 +1,215 @@
+"""Low-rank adapters of many requests at once beside a shared projection, and
+their backward pass, for the linears of `ltx_ops`. No counterpart in the
+reference.
+
+x (..., K) and y (..., N) are read as rows; rows segment_starts[s] ..
+segment_starts[s + 1] - 1 belong to request s and take adapter
+segment_adapters[s] (one outside 0 .. L - 1 is none; rows outside all segments
+have none). Adapter l is a[l] [r, K], b[l] [N, r], scale[l]:
+
+    y' = y + scale (x a^T) b^T
+    dx = scale (dy b) a,  da = scale (dy b)^T x,  db = scale dy^T (x a^T)
+
+with da and db summed over an adapter's rows, in a fixed order. The segments
+stay on the device: nothing synchronises. Starts have to rise; the kernels
+stay within the tensors whatever they hold.
+
+On the GPU these run oga_lora_add and oga_lora_bwd on torch's current stream:
+bf16 or fp16, r a multiple of 8 up to 128, K and N multiples of 8. Other
+inputs take the same formulas in torch, in float32; under
+OPENGENIE_AMD_STRICT=1 a GPU input that would do so raises. Tensors that do not
+fit each other raise ValueError.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from ._launch import bytes_on, call_on, rows_layout
+from .ltx_ops import _fallback, _hip, _xdt, fp8_linear_forward
+
+__all__ = ["LoraAdapters", "lora_add", "lora_backward", "lora_add_with_grad", "fp8_linear_lora_forward"]
+
+
+@dataclass
+class LoraAdapters:
+    """Adapters of one projection: a [L, r, K], b [L, N, r], scale [L] float32
+    (None: 1)."""
+    a: torch.Tensor
+    b: torch.Tensor
+    scale: torch.Tensor | None = None
+
+    @staticmethod
+    def stack(adapters: list[tuple[torch.Tensor, torch.Tensor, float]]) -> "LoraAdapters":
+        """From (a [r, K], b [N, r], scale) of each adapter; smaller ranks are
+        filled up with zeros to the largest one, to a multiple of 8."""
+        rank = max((a.shape[0] + 7) // 8 * 8 for a, _, _ in adapters)
+        pad = torch.nn.functional.pad
+        return LoraAdapters(torch.stack([pad(a, (0, 0, 0, rank - a.shape[0])) for a, _, _ in adapters]),
+                            torch.stack([pad(b, (0, rank - b.shape[1])) for _, b, _ in adapters]),
+                            torch.tensor([float(s) for _, _, s in adapters], device=adapters[0][0].device))
+
+
+def _check(x, n, a, b, scale, starts, ids) -> None:
+    if a.ndim != 3 or b.ndim != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or not a.numel():
+        raise ValueError(f"adapters a {tuple(a.shape)}, b {tuple(b.shape)}")
+    if a.shape[2] != x.shape[-1] or b.shape[1] != n:
+        raise ValueError(f"adapters a {tuple(a.shape)}, b {tuple(b.shape)} for {x.shape[-1]} -> {n}")
+    if a.dtype != x.dtype or b.dtype != x.dtype or not x.is_floating_point():
+        raise ValueError(f"dtypes x {x.dtype}, a {a.dtype}, b {b.dtype}")
+    if scale is not None and (scale.shape != a.shape[:1] or scale.dtype != torch.float32):
+        raise ValueError(f"scale {scale.dtype} {tuple(scale.shape)} of {a.shape[0]} adapters")
+    if (starts.ndim != 1 or ids.ndim != 1 or starts.shape[0] != ids.shape[0] + 1
+            or starts.dtype not in (torch.int32, torch.int64) or ids.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"segments: starts {starts.dtype} {tuple(starts.shape)}, adapters {ids.dtype} "
+                         f"{tuple(ids.shape)}")
+    if any(t is not None and t.device != x.device for t in (a, b, scale, starts, ids)):
+        raise ValueError("adapter inputs on different devices")
+
+
+def _kernel_ok(x, n, a) -> bool:
+    return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and a.shape[1] % 8 == 0 and a.shape[1] <= 128
+            and x.shape[-1] % 8 == 0 and n % 8 == 0 and a.shape[0] <= 2000)
+
+
+def _i32(t: torch.Tensor, most: int) -> torch.Tensor:
+    if t.dtype != torch.int32:
+        t = t.clamp(-1, most).to(torch.int32)
+    return t.contiguous()
+
+
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _torch_rows(x, a, starts, ids, scale):
+    """For each row and adapter whether the row takes it [T, L], and the scale
+    of each of the L r ranks."""
+    row = torch.arange(x.shape[0], device=x.device)
+    seg = torch.searchsorted(starts.long().contiguous(), row, right=True) - 1
+    inside = (seg >= 0) & (seg < ids.shape[0])
+    mine = torch.where(inside, ids.long()[seg.clamp(0, max(ids.shape[0] - 1, 0))], -1) if ids.shape[0] else row * 0 - 1
+    keep = mine[:, None] == torch.arange(a.shape[0], device=x.device)
+    s = torch.ones(a.shape[0], device=x.device) if scale is None else scale
+    return keep.repeat_interleave(a.shape[1], 1), s.repeat_interleave(a.shape[1])
+
+
+def _torch_low(x, w, keep, s):
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    return torch.where(keep, torch.matmul(x.to(wide), w.to(wide)) * s.to(wide), 0.0)
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor | None,
+             segment_starts: torch.Tensor, segment_adapters: torch.Tensor, *, out: torch.Tensor | None = None,
+             save_low: bool = False):
+    """y + scale (x a^T) b^T row by row, into `out` (which may be y) or a new
+    tensor; with `save_low` also the rows' scale (x a^T), which
+    `lora_backward` reads."""
+    _check(x, y.shape[-1], a, b, scale, segment_starts, segment_adapters)
+    if y.shape[:-1] != x.shape[:-1] or y.dtype != x.dtype or y.device != x.device:
+        raise ValueError(f"y {y.dtype} {tuple(y.shape)} for x {x.dtype} {tuple(x.shape)}")
+    if out is not None and (out.shape != y.shape or out.dtype != y.dtype or out.device != y.device
+                            or not out.is_contiguous()):
+        raise ValueError(f"out {out.dtype} {tuple(out.shape)} for y {y.dtype} {tuple(y.shape)}, contiguous")
+    n, k, rank = y.shape[-1], x.shape[-1], a.shape[1]
+    rows = x.numel() // k if k else 0
+    if rows == 0 or segment_adapters.shape[0] == 0:
+        r = y.clone(memory_format=torch.contiguous_format) if out is None else out if out is y else out.copy_(y)
+        return (r, torch.zeros((rows, rank), device=x.device, dtype=torch.float32)) if save_low else r
+    if not _kernel_ok(x, n, a) or (out is not None and out.data_ptr() % 16):
+        _fallback("lora_add", y, x)
+        x2 = x.reshape(-1, k)
+        keep, s = _torch_rows(x2, a, segment_starts, segment_adapters, scale)
+        low = _torch_low(x2, a.flatten(0, 1).t(), keep, s)
+        r = y.reshape(-1, n).to(low.dtype) + torch.matmul(low, b.to(low.dtype).transpose(1, 2).flatten(0, 1))
+        r = r.to(y.dtype).reshape(y.shape)
+        r = r if out is None else out.copy_(r)
+        return (r, low.reshape(rows, -1, rank).sum(1)) if save_low else r
+    if out is None:
+        out = torch.empty(y.shape, device=y.device, dtype=y.dtype)
+    x2, xs = rows_layout(x)
+    y2, ys = rows_layout(y)
+    low = torch.empty((rows, rank), device=x.device, dtype=torch.float32)
+    a, b = _packed(a), _packed(b)
+    scale = None if scale is None else scale.contiguous()
+    starts, ids = _i32(segment_starts, rows), _i32(segment_adapters, a.shape[0])
+    _hip("lora_add")
+    call_on(x, "oga_lora_add", _xdt(x), y2.data_ptr(), ys, x2.data_ptr(), xs, a.data_ptr(), b.data_ptr(),
+            None if scale is None else scale.data_ptr(), starts.data_ptr(), ids.data_ptr(), ids.shape[0], a.shape[0],
+            low.data_ptr(), out.data_ptr(), n, rows, k, n, rank)
+    return (out, low) if save_low else out
+
+
+def lora_backward(dy: torch.Tensor, x: torch.Tensor, low: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                  scale: torch.Tensor | None, segment_starts: torch.Tensor, segment_adapters: torch.Tensor):
+    """dx, da, db of `lora_add` with these inputs from its output's gradient
+    and the `low` it saved (y's gradient is dy)."""
+    n, k, rank = dy.shape[-1], x.shape[-1], a.shape[1]
+    _check(x, n, a, b, scale, segment_starts, segment_adapters)
+    if dy.shape[:-1] != x.shape[:-1] or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError(f"dy {dy.dtype} {tuple(dy.shape)} for x {x.dtype} {tuple(x.shape)}")
+    rows = x.numel() // k if k else 0
+    if low.shape != (rows, rank) or low.device != x.device or not low.is_floating_point():
+        raise ValueError(f"low {low.dtype} {tuple(low.shape)} of {rows} rows, rank {rank}")
+    if rows == 0 or segment_adapters.shape[0] == 0:
+        return torch.zeros(x.shape, device=x.device, dtype=x.dtype), torch.zeros_like(a), torch.zeros_like(b)
+    if not _kernel_ok(x, n, a) or low.dtype != torch.float32:
+        _fallback("lora_backward", dy, x)
+        x2, dy2 = x.reshape(-1, k), dy.reshape(-1, n)
+        keep, s = _torch_rows(x2, a, segment_starts, segment_adapters, scale)
+        dlow = _torch_low(dy2, b.transpose(1, 2).flatten(0, 1).t(), keep, s)
+        mine = torch.where(keep, low.to(dlow.dtype).repeat(1, a.shape[0]), 0.0)
+        some = keep.any(1, keepdim=True)
+        xf, df = (torch.where(some, t.to(dlow.dtype), 0.0) for t in (x2, dy2))
+        dx = torch.matmul(dlow, a.to(dlow.dtype).flatten(0, 1)).to(x.dtype).reshape(x.shape)
+        da = torch.matmul(dlow.t(), xf).reshape(a.shape).to(a.dtype)
+        db = torch.matmul(mine.t(), df).reshape(a.shape[0], rank, n).transpose(1, 2).contiguous().to(b.dtype)
+        return dx, da, db
+    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    x2, xs = rows_layout(x)
+    dy2, dys = rows_layout(dy)
+    low, a, b = _packed(low), _packed(a), _packed(b)
+    scale = None if scale is None else scale.contiguous()
+    starts, ids = _i32(segment_starts, rows), _i32(segment_adapters, a.shape[0])
+    da, db = torch.empty_like(a), torch.empty_like(b)
+    size = bytes_on(x, "oga_lora_bwd_workspace_bytes", rows, k, n, rank, a.shape[0])
+    ws = torch.empty((size,), device=x.device, dtype=torch.uint8)
+    _hip("lora_backward")
+    call_on(x, "oga_lora_bwd", _xdt(x), dy2.data_ptr(), dys, x2.data_ptr(), xs, low.data_ptr(), a.data_ptr(),
+            b.data_ptr(), None if scale is None else scale.data_ptr(), starts.data_ptr(), ids.data_ptr(),
+            ids.shape[0], a.shape[0], dx.data_ptr(), k, da.data_ptr(), db.data_ptr(), rows, k, n, rank, ws.data_ptr(),
+            size)
+    return dx, da, db
+
+
+class _LoraAdd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, x, a, b, scale, segment_starts, segment_adapters):
+        r, low = lora_add(y, x, a, b, scale, segment_starts, segment_adapters, save_low=True)
+        ctx.save_for_backward(x, low, a, b, scale, segment_starts, segment_adapters)
+        return r
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, low, a, b, scale, starts, ids = ctx.saved_tensors
+        return (dy, *lora_backward(dy, x, low, a, b, scale, starts, ids), None, None, None)
+
+
+def lora_add_with_grad(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                       scale: torch.Tensor | None, segment_starts: torch.Tensor,
+                       segment_adapters: torch.Tensor) -> torch.Tensor:
+    """`lora_add`, differentiable in y, x, a and b."""
+    return _LoraAdd.apply(y, x, a, b, scale, segment_starts, segment_adapters)
+
+
+def fp8_linear_lora_forward(module, x: torch.Tensor, adapters: LoraAdapters, segment_starts: torch.Tensor,
+                            segment_adapters: torch.Tensor) -> torch.Tensor:
+    """`ltx_ops.fp8_linear_forward(module, x)` with the requests' adapters
+    added to its output in place."""
+    y = fp8_linear_forward(module, x)
+    return lora_add(y, x, adapters.a, adapters.b, adapters.scale, segment_starts, segment_adapters,
+                    out=y if y.is_contiguous() else None)

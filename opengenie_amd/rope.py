@@ -12,6 +12,8 @@ frequency times the token's coordinate on the axis.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 
@@ -31,3 +33,34 @@ def video_rope_cos_sin(grid: tuple[int, int, int], *, heads: int = 32, head_dim:
     ang = pos[:, axis] * freq  # (N, nfreq)
     ang = ang.reshape(-1, heads, half).transpose(0, 1).unsqueeze(0)  # (1, heads, N, half)
     return ang.cos().to(dtype).contiguous(), ang.sin().to(dtype).contiguous()
+
+
+def rotary_cos_sin(length: int, rotary_dim: int, *, theta: float = 10000.0, start: int = 0, scaling: str | None = None,
+                   factor: float = 1.0, original_length: int | None = None, fast: float = 32.0, slow: float = 1.0,
+                   device: str | torch.device = "cpu", dtype: torch.dtype = torch.float32):
+    """cos, sin of shape (length, rotary_dim // 2) for the positions start ..
+    start + length - 1 of a sequence, shared by all heads (`head_rope`): plane
+    i turns by theta**(-2i / rotary_dim) a position. Angles are float64, so far
+    positions keep theirs. For contexts `factor` times longer than a model was
+    trained on, scaling "linear" divides the positions by the factor; "ntk"
+    stretches the base by factor**(rotary_dim / (rotary_dim - 2)), which slows
+    the slowest plane by the factor and leaves the fastest; "ramp" divides a
+    plane's angle where it turns fewer than `slow` times over original_length
+    positions, keeps it where it turns more than `fast` times, and mixes the
+    two linearly in the number of turns between."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim {rotary_dim}")
+    if scaling not in (None, "linear", "ntk", "ramp") or (scaling is None and factor != 1.0):
+        raise ValueError(f"scaling {scaling} by {factor}")
+    if scaling == "ramp" and (original_length is None or not fast > slow):
+        raise ValueError("ramp scaling needs original_length and fast > slow")
+    if scaling == "ntk" and rotary_dim > 2:
+        theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    freq = theta ** (-torch.arange(0, rotary_dim, 2, device=device, dtype=torch.float64) / rotary_dim)
+    if scaling == "linear":
+        freq = freq / factor
+    elif scaling == "ramp":
+        keep = ((original_length * freq / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+        freq = freq * keep + freq / factor * (1 - keep)
+    ang = torch.arange(start, start + length, device=device, dtype=torch.float64)[:, None] * freq
+    return ang.cos().to(dtype), ang.sin().to(dtype)
