@@ -454,15 +454,18 @@ int64_t oga_rows_per_wave(int kind, int64_t batch, int64_t tokens, int64_t cols)
  * sees no key has o = 0, lse = -inf and no gradient. Scores and sums are
  * float32, P and dS round to bf16 for the second products, results once.
  * Nothing is summed by atomics: the same call gives the same bits.
- * The backward pass needs a 256-byte aligned workspace of
- * oga_attention_bwd_workspace_bytes(...) bytes on the current device.
+ * Workspaces (256-byte aligned) of the queries' bytes on the current device;
+ * the forward pass needs none where its query is 0.
  */
+int64_t oga_attention_lse_workspace_bytes(int64_t batch, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads,
+                                          int64_t head_dim, int causal);
 int oga_attention_lse(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
                       const void* v, const int64_t v_strides[3], void* o, const int64_t o_strides[3], float* lse,
                       int64_t batch, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads, int64_t head_dim,
-                      float softmax_scale, int causal, const int32_t* k_lens, void* stream);
+                      float softmax_scale, int causal, const int32_t* k_lens, void* workspace,
+                      int64_t workspace_bytes, void* stream);
 int64_t oga_attention_bwd_workspace_bytes(int64_t batch, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads,
-                                          int64_t head_dim);
+                                          int64_t head_dim, int causal);
 int oga_attention_bwd(const void* dout, const int64_t do_strides[3], const void* q, const int64_t q_strides[3],
                       const void* k, const int64_t k_strides[3], const void* v, const int64_t v_strides[3],
                       const void* out, const int64_t o_strides[3], const float* lse, void* dq,

@@ -101,9 +101,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "oga_rows_per_wave": (_i64, [_i32, _i64, _i64, _i64]),
     "oga_fp8_per_head_noalloc_max_bytes": (_i64, []),
     "oga_fp8_quantize_per_head_noalloc": (_i32, [_p, _i32, _p, _p, _i64, _i64, _i64, _i64, _p]),
+    "oga_attention_lse_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i32]),
     "oga_attention_lse": (_i32, [_p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64, _i64, _i64, _i64, _i64, _i64,
-                                 _f32, _i32, _p, _p]),
-    "oga_attention_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
+                                 _f32, _i32, _p, _p, _i64, _p]),
+    "oga_attention_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i32]),
     "oga_attention_bwd": (_i32, [_p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _p, _i64p, _p, _i64p, _p,
                                  _i64p, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _p, _p, _i64, _p]),
     "oga_head_rmsnorm_rope": (_i32, [_i32, _p, _i64p, _p, _i64p, _p, _p, _i32, _p, _p, _i32, _i64, _i64, _p, _i32,

@@ -134,10 +134,12 @@ def flash_attn_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_sc
     lens = _lens32(k_lens, nk)
     out = torch.empty((b, nq, h, d), device=q.device, dtype=torch.bfloat16)
     lse = torch.empty((b, h, nq), device=q.device, dtype=torch.float32)
+    size = bytes_on(q, "oga_attention_lse_workspace_bytes", b, nq, nk, h, hk, d, int(causal))
+    ws = torch.empty((size,), device=q.device, dtype=torch.uint8) if size else None
     _hip("flash_attn_lse")
     call_on(q, "oga_attention_lse", q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(),
             (nq * h * d, h * d, d), lse.data_ptr(), b, nq, nk, h, hk, d, scale, int(causal),
-            None if lens is None else lens.data_ptr())
+            None if lens is None else lens.data_ptr(), None if ws is None else ws.data_ptr(), size)
     return out, lse
 
 
@@ -167,7 +169,7 @@ def flash_attn_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v:
     dk = torch.empty((b, nk, hk, d), device=q.device, dtype=torch.bfloat16)
     dv = torch.empty_like(dk)
     dqs, dks = (nq * h * d, h * d, d), (nk * hk * d, hk * d, d)
-    size = bytes_on(q, "oga_attention_bwd_workspace_bytes", b, nq, nk, h, hk, d)
+    size = bytes_on(q, "oga_attention_bwd_workspace_bytes", b, nq, nk, h, hk, d, int(causal))
     ws = torch.empty((size,), device=q.device, dtype=torch.uint8)
     _hip("flash_attn_backward")
     call_on(q, "oga_attention_bwd", dout.data_ptr(), ds, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,

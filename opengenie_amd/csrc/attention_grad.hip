@@ -28,7 +28,6 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kGT = 64;    // rows of a tile
-constexpr int kGBufs = 3;  // tile pairs in the ring
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnGradArgs {
@@ -37,13 +36,15 @@ struct AttnGradArgs {
   int64_t q_s[3], k_s[3], v_s[3], do_s[3], o_s[3], dq_s[3], dk_s[3], dv_s[3];  // (batch, token, head); unit along D
   float* lse;          // [B, H, Nq]
   float* ld;           // [B, H, ceil(Nq / 64)][64 lse2 | 64 Delta] (backward)
-  float* part;         // dk/dv parts: [splits][dk | dv][B, Hk, Nk, D]
+  float* part;         // what the parts of split blocks leave, float32
+  float* part_ml;      // k_attn_lse: their running maxima and sums
   const int32_t* k_lens;
   int64_t nq, nk, batch;
   int heads, kv_heads, group;
   int blocks;          // query (key) blocks per (batch, head)
   int causal;
-  int splits;          // parts of a key block's query steps
+  int64_t nfull;       // blocks run whole; the others run as ksplit parts of their steps
+  int ksplit;
   float scale, scale_log2;
 };
 
@@ -58,20 +59,62 @@ OGA_DEVICE int64_t xcd_order(uint32_t block, uint32_t grid) {
   return (int64_t)xcd * per + min(xcd, extra) + (block >> 3);
 }
 
+// The block a workgroup works on: blocks 0 .. nfull - 1 whole, later ones in
+// ksplit parts (part -1: whole). Blocks that would fill only part of a last
+// round of the CUs (or of the only one) are cut, and a join adds the parts up.
+struct GradUnit {
+  int64_t wg;
+  int part;
+};
+OGA_DEVICE GradUnit grad_unit(const AttnGradArgs& a) {
+  if ((int64_t)blockIdx.x < a.nfull) return {xcd_order(blockIdx.x, (uint32_t)a.nfull), -1};
+  const uint32_t u = blockIdx.x - (uint32_t)a.nfull;
+  return {a.nfull + u / (uint32_t)a.ksplit, (int)(u % (uint32_t)a.ksplit)};
+}
+
 // ------------------------------------------------------------- LDS tiles
 // Row r of a tile (2 D bytes, D / 8 chunks of 16) keeps chunk c at c ^ sw(r).
 // Two orders, by how the kernel reads: 32-row fragments (32x32x16 MFMA) with
 // transposing reads of 4 rows x 64 bytes, or 16-row fragments (16x16x32) with
-// transposing reads of 8 rows x 32 bytes; each read's lanes then cover all
-// banks once.
+// transposing reads of 8 rows x 32 bytes. A ds_read_b128 is served 16 lanes at
+// a time, lanes 0-3, 12-15, 20-23, 24-27 together (and 4-11, 16-19, 28-31),
+// which for a 16-row fragment are rows 0-3, 12-15 of one chunk and 4-11 of the
+// next one: sw16 keeps the two chunks of a pair apart for those rows, and for
+// the 8 rows of a transposing read (checked below).
 template <int D>
 constexpr int sw32(int r) {
   return D == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
 }
 template <int D>
 constexpr int sw16(int r) {
-  return D == 128 ? ((r & 7) << 1) | ((r >> 3) & 1) : (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
+  return D == 128 ? (((r & 7) ^ ((r >> 1) & 4)) << 1) | ((r >> 3) & 1)
+                  : ((((r >> 1) & 3) ^ ((r >> 2) & 2)) << 1) | ((r >> 3) & 1);
 }
+
+template <int D>
+constexpr bool frag16_conflict_free() {
+  for (int s = 0; s < D / 32; ++s)
+    for (int half = 0; half < 2; ++half)
+      for (int first = 0; first < 2; ++first) {
+        unsigned seen = 0;  // 16-byte columns of the 256 bytes of all banks
+        for (int l = 0; l < 32; ++l) {
+          const bool in = l < 4 || (l >= 12 && l < 16) || (l >= 20 && l < 28);
+          if (in != (first == 0)) continue;
+          const int r = l & 15, c = 4 * s + 2 * half + (l >> 4);
+          seen |= 1u << ((r * (D / 8) + (c ^ sw16<D>(r))) & 15);
+        }
+        if (seen != 0xFFFF) return false;
+      }
+  for (int d = 0; d < D / 16; ++d)
+    for (int r0 = 0; r0 < 16; r0 += 8) {
+      unsigned seen = 0;
+      for (int r = r0; r < r0 + 8; ++r)
+        for (int c = 2 * d; c < 2 * d + 2; ++c) seen |= 1u << ((r * (D / 8) + (c ^ sw16<D>(r))) & 15);
+      if (seen != 0xFFFF) return false;
+    }
+  return true;
+}
+static_assert(frag16_conflict_free<64>() && frag16_conflict_free<128>(), "fragment reads would conflict");
 
 template <int OFF>
 OGA_DEVICE bf16x8 rd_b128(uint32_t addr) {
@@ -158,17 +201,18 @@ OGA_DEVICE float sum_halves(float v) {
 // W waves of 32 queries. S^T = K Q^T in 32 x 32 blocks (lane l: query l % 32,
 // keys 8g + 4 (l / 32) + r), online softmax in base 2 with the running max
 // moved only when a score passes it by 8 (P stays below 2^8), O^T += V^T P^T.
-template <int D, int W, bool CAUSAL>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attn_lse(AttnGradArgs a) {
+template <int D, int W, int BUFS, bool CAUSAL>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void k_attn_lse(
+    AttnGradArgs a) {
   constexpr int kTile = kGT * D * 2, kPair = 2 * kTile, NS = D / 16, ND = D / 32;
   typedef TileDma<D, W, false> Dma;
-  __shared__ uint4 smem[kGBufs * kPair / 16];
+  __shared__ uint4 smem[BUFS * kPair / 16];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int64_t wg = xcd_order(blockIdx.x, gridDim.x);
-  int qb = (int)(wg % a.blocks);
+  const GradUnit unit = grad_unit(a);
+  int qb = (int)(unit.wg % a.blocks);
   if (CAUSAL) qb = a.blocks - 1 - qb;  // the longest first
-  const int64_t bh = wg / a.blocks;
+  const int64_t bh = unit.wg / a.blocks;
   const int h = (int)(bh % a.heads);
   const int64_t b = bh / a.heads;
   const int hk = h / a.group;
@@ -179,6 +223,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
   int64_t kend = nkb;
   if (CAUSAL) kend = min(nkb, max((int64_t)0, min((int64_t)(qb + 1) * 32 * W, a.nq) + shift));
   const int nsteps = (int)((kend + kGT - 1) / kGT);
+  const int st0 = unit.part < 0 ? 0 : (int)((int64_t)nsteps * unit.part / a.ksplit);
+  const int st1 = unit.part < 0 ? nsteps : (int)((int64_t)nsteps * (unit.part + 1) / a.ksplit);
 
   bf16x8 qf[NS];
   {
@@ -211,8 +257,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
 
   auto step = [&](auto slot_c, int st) {
     constexpr int SLOT = decltype(slot_c)::value, BASE = SLOT * kPair;
-    ring_wait<2 * Dma::kDI>();
-    dma(min(st + 2, nsteps - 1), (SLOT + 2) % kGBufs);
+    ring_wait<BUFS == 3 ? 2 * Dma::kDI : 0>();
+    if (BUFS == 3 || st + 1 < st1) dma(min(st + BUFS - 1, st1 - 1), (SLOT + BUFS - 1) % BUFS);
+    // a wave behind the last query, or whose queries see none of these keys
+    if (q0 >= a.nq || (CAUSAL && (int64_t)st * kGT > q0 + 31 + shift)) return;
     f32x16 s[2];
     auto block = [&](auto j_c) {
       constexpr int OFF = BASE + 32 * 2 * D * decltype(j_c)::value;
@@ -312,19 +360,32 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     pv(IC<3>{}, v1, v0);
   };
 
-  if (nsteps > 0) {  // (uniform over the workgroup)
-    dma(0, 0);
-    dma(min(1, nsteps - 1), 1);
-    for (int st = 0; st < nsteps; st += 3) {
+  if (st1 > st0) {  // (uniform over the workgroup)
+    dma(st0, 0);
+    if (BUFS == 3) dma(min(st0 + 1, st1 - 1), 1);
+    for (int st = st0; st < st1; st += BUFS) {
       step(IC<0>{}, st);
-      if (st + 1 < nsteps) step(IC<1>{}, st + 1);
-      if (st + 2 < nsteps) step(IC<2>{}, st + 2);
+      if (st + 1 < st1) step(IC<1>{}, st + 1);
+      if constexpr (BUFS == 3)
+        if (st + 2 < st1) step(IC<2 % BUFS>{}, st + 2);
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
   const float l = sum_halves(l_run);
-  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // no key: 0; NaN stays
+  if (unit.part >= 0) {  // O^T unnormalized, with m and l (every wave takes this branch)
+    const int64_t row = (int64_t)(blockIdx.x - a.nfull) * 32 * W + wv * 32 + ql;
+    float* po = a.part + row * D;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(float4*)(po + 32 * d + 8 * g + 4 * hl) =
+            make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+    if (hl == 0) *(float2*)(a.part_ml + 2 * row) = make_float2(m_run, l);
+    return;
+  }
+  const float inv = l > 0.0f ? 1.0f / l : l;  // no key: 0; NaN stays
   const int64_t qi = q0 + ql;
   if (hl == 0 && qi < a.nq)
     a.lse[bh * a.nq + qi] = l == 0.0f ? -INFINITY : m_run * kLn2 + logf(l);
@@ -351,6 +412,42 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2))) 
     const uint4 w = *(const uint4*)(ot + r * 2 * D + ((oc ^ (r % kLpr)) << 4));
     if (q0 + r < a.nq) *(uint4*)(ob + (q0 + r) * a.o_s[1]) = w;
   }
+}
+
+// out and lse of the blocks that ran in parts: O = sum 2^(m_p - M) O_p / L,
+// L = sum 2^(m_p - M) l_p. D / 8 lanes a row.
+template <int D, int ROWS>
+__global__ __launch_bounds__(256) void k_attn_lse_join(AttnGradArgs a) {
+  constexpr int kLpr = D / 8;
+  const int64_t r = (int64_t)blockIdx.x * (256 / kLpr) + threadIdx.x / kLpr;  // (split block, row)
+  const int64_t blk = r / ROWS, wg = a.nfull + blk;
+  if (wg >= a.batch * a.heads * a.blocks) return;
+  int qb = (int)(wg % a.blocks);
+  if (a.causal) qb = a.blocks - 1 - qb;
+  const int64_t bh = wg / a.blocks, row = r - blk * ROWS, qi = (int64_t)qb * ROWS + row;
+  if (qi >= a.nq) return;
+  const int c = threadIdx.x % kLpr;
+  const int64_t first = blk * a.ksplit * ROWS + row;
+  float m = -INFINITY;
+  for (int p = 0; p < a.ksplit; ++p) m = __builtin_fmaxf(m, a.part_ml[2 * (first + p * ROWS)]);
+  const float nm = m == -INFINITY ? 0.0f : -m;
+  float l = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int p = 0; p < a.ksplit; ++p) {
+    const int64_t at = first + p * ROWS;
+    const float2 ml = *(const float2*)(a.part_ml + 2 * at);
+    const float w = __builtin_amdgcn_exp2f(ml.x + nm);
+    l = fmaf(w, ml.y, l);
+    const float* f = a.part + at * D + 8 * c;
+    const float4 u = *(const float4*)f, v = *(const float4*)(f + 4);
+    o[0] = fmaf(w, u.x, o[0]), o[1] = fmaf(w, u.y, o[1]), o[2] = fmaf(w, u.z, o[2]), o[3] = fmaf(w, u.w, o[3]);
+    o[4] = fmaf(w, v.x, o[4]), o[5] = fmaf(w, v.y, o[5]), o[6] = fmaf(w, v.z, o[6]), o[7] = fmaf(w, v.w, o[7]);
+  }
+  const float inv = l > 0.0f ? 1.0f / l : l;  // no key: 0; NaN stays
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] *= inv;
+  const int64_t b = bh / a.heads, h = bh - b * a.heads;
+  *(uint4*)(a.o + b * a.o_s[0] + qi * a.o_s[1] + h * a.o_s[2] + 8 * c) = pack8(o);
+  if (c == 0) a.lse[bh * a.nq + qi] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
 }
 
 // --------------------------------------------------- Delta and base-2 lse
@@ -392,28 +489,30 @@ __global__ __launch_bounds__(256) void k_attn_delta(AttnGradArgs a) {
 // reads, whose 32 keys' order (4 (l / 16) + r of two 16-key blocks) is that of
 // the blocks' accumulators. 16x16x32 MFMAs draw less power than 32x32x16 at
 // the same rate, and no row maximum is needed here.
-constexpr int kGW = 8;
-template <int D, bool CAUSAL>
-__global__ __launch_bounds__(64 * kGW) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attn_dq(AttnGradArgs a) {
+template <int D, int W, int BUFS, bool CAUSAL>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void k_attn_dq(
+    AttnGradArgs a) {
   constexpr int kTile = kGT * D * 2, kPair = 2 * kTile, NS = D / 32, ND = D / 16;
-  typedef TileDma<D, kGW, true> Dma;
-  __shared__ uint4 smem[kGBufs * kPair / 16];
+  typedef TileDma<D, W, true> Dma;
+  __shared__ uint4 smem[BUFS * kPair / 16];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int64_t wg = xcd_order(blockIdx.x, gridDim.x);
-  int qb = (int)(wg % a.blocks);
+  const GradUnit unit = grad_unit(a);
+  int qb = (int)(unit.wg % a.blocks);
   if (CAUSAL) qb = a.blocks - 1 - qb;
-  const int64_t bh = wg / a.blocks;
+  const int64_t bh = unit.wg / a.blocks;
   const int h = (int)(bh % a.heads);
   const int64_t b = bh / a.heads;
   const int hk = h / a.group;
   const int c16 = lane & 15, kg = lane >> 4;
-  const int64_t q0 = (int64_t)qb * 32 * kGW + wv * 32;
+  const int64_t q0 = (int64_t)qb * 32 * W + wv * 32;
   const int64_t nkb = key_count(a, b);
   const int64_t shift = nkb - a.nq;
   int64_t kend = nkb;
-  if (CAUSAL) kend = min(nkb, max((int64_t)0, min((int64_t)(qb + 1) * 32 * kGW, a.nq) + shift));
+  if (CAUSAL) kend = min(nkb, max((int64_t)0, min((int64_t)(qb + 1) * 32 * W, a.nq) + shift));
   const int nsteps = (int)((kend + kGT - 1) / kGT);
+  const int st0 = unit.part < 0 ? 0 : (int)((int64_t)nsteps * unit.part / a.ksplit);
+  const int st1 = unit.part < 0 ? nsteps : (int)((int64_t)nsteps * (unit.part + 1) / a.ksplit);
 
   bf16x8 qf[2][NS], gf[2][NS];  // Q and dO, B operands: query 16 i + c16, d = 32 s + 8 kg ..
   float lse2[2], delta[2];
@@ -453,8 +552,9 @@ __global__ __launch_bounds__(64 * kGW) __attribute__((amdgpu_waves_per_eu(2, 2))
   const uint32_t ta = lds0 + (4 * kg + j4) * (2 * D) + (((a4 >> 1) ^ sw16<D>(4 * kg + j4)) << 4) + (a4 & 1) * 8;
 
   auto step = [&](uint32_t base, int slot2, int st) {
-    ring_wait<2 * Dma::kDI>();
-    dma(min(st + 2, nsteps - 1), slot2);
+    ring_wait<BUFS == 3 ? 2 * Dma::kDI : 0>();
+    if (BUFS == 3 || st + 1 < st1) dma(min(st + BUFS - 1, st1 - 1), slot2);
+    if (q0 >= a.nq || (CAUSAL && (int64_t)st * kGT > q0 + 31 + shift)) return;
     const int64_t key0 = (int64_t)st * kGT;
     const bool edge = CAUSAL ? key0 + kGT > min(nkb, q0 + shift + 1) : key0 + kGT > nkb;
     auto half = [&](auto j_c) {  // keys 32 j .. + 31 of the tile
@@ -536,17 +636,25 @@ __global__ __launch_bounds__(64 * kGW) __attribute__((amdgpu_waves_per_eu(2, 2))
     half(IC<0>{});
     half(IC<1>{});
   };
-  if (nsteps > 0) {
-    dma(0, 0);
-    dma(min(1, nsteps - 1), 1);
+  if (st1 > st0) {
+    dma(st0, 0);
+    if (BUFS == 3) dma(min(st0 + 1, st1 - 1), 1);
     int slot = 0;
-    for (int st = 0; st < nsteps; ++st) {
-      step(slot * kPair, slot == 0 ? 2 : slot - 1, st);
-      slot = slot == 2 ? 0 : slot + 1;
+    for (int st = st0; st < st1; ++st) {
+      step(slot * kPair, slot == 0 ? BUFS - 1 : slot - 1, st);
+      slot = slot == BUFS - 1 ? 0 : slot + 1;
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   // lane: query 16 i + c16, d = 16 db + 4 kg .. + 3
+  if (unit.part >= 0) {
+    float* o = a.part + ((int64_t)(blockIdx.x - a.nfull) * 32 * W + wv * 32 + c16) * D + 4 * kg;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) *(f32x4*)(o + 16 * i * D + 16 * d) = acc[d][i] * a.scale;
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int64_t qi = q0 + 16 * i + c16;
@@ -565,29 +673,22 @@ __global__ __launch_bounds__(64 * kGW) __attribute__((amdgpu_waves_per_eu(2, 2))
 // 16 x 16 blocks (lane l: key l % 16, queries 4 (l / 16) + r), whose lse and
 // Delta come from LDS, four queries a read; dv^T += dO^T P and dk^T += Q^T dS
 // with the transposed tiles by transposing reads.
-template <int D>
-struct DkvShape {
-  static constexpr int kW = 8;   // waves
-  static constexpr int kKB = 2;  // 16-key blocks per wave
-  static constexpr int kKeys = 16 * kW * kKB;   // keys per workgroup
-};
-template <int D, bool CAUSAL>
-__global__ __launch_bounds__(64 * DkvShape<D>::kW) __attribute__((amdgpu_waves_per_eu(DkvShape<D>::kW / 4, DkvShape<D>::kW / 4))) void k_attn_dkv(AttnGradArgs a) {
+template <int D, int W, int BUFS, bool CAUSAL>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void k_attn_dkv(
+    AttnGradArgs a) {
   constexpr int kTile = kGT * D * 2, kPair = 2 * kTile + 512, NS = D / 32, ND = D / 16;
-  constexpr int W = DkvShape<D>::kW, KB = DkvShape<D>::kKB, kKeys = DkvShape<D>::kKeys;
+  constexpr int KB = 2, kKeys = 32 * W;
   typedef TileDma<D, W, true> Dma;
-  __shared__ uint4 smem[kGBufs * kPair / 16];
+  __shared__ uint4 smem[BUFS * kPair / 16];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int64_t unit = xcd_order(blockIdx.x, gridDim.x);
-  const int part = (int)(unit % a.splits);
-  const int64_t wg = unit / a.splits;
-  const int kblk = (int)(wg % a.blocks);
-  const int64_t bh = wg / a.blocks;
+  const GradUnit unit = grad_unit(a);
+  const int kblk = (int)(unit.wg % a.blocks);
+  const int64_t bh = unit.wg / a.blocks;
   const int hk = (int)(bh % a.kv_heads);
   const int64_t b = bh / a.kv_heads;
   const int c16 = lane & 15, kg = lane >> 4;
-  const int64_t kblk0 = (int64_t)kblk * kKeys, k0 = kblk0 + wv * 16 * KB;
+  const int64_t kblk0 = (int64_t)kblk * kKeys, k0 = kblk0 + wv * 32;
   const int64_t nkb = key_count(a, b);
   const int64_t shift = nkb - a.nq;
   const int nqt = (int)((a.nq + kGT - 1) / kGT);
@@ -598,7 +699,8 @@ __global__ __launch_bounds__(64 * DkvShape<D>::kW) __attribute__((amdgpu_waves_p
   if (kblk0 >= nkb) t0 = nqt;
   const int per = nqt - t0;
   const int64_t all = (int64_t)per * a.group;
-  const int s0 = (int)(all * part / a.splits), s1 = (int)(all * (part + 1) / a.splits);
+  const int s0 = unit.part < 0 ? 0 : (int)(all * unit.part / a.ksplit);
+  const int s1 = unit.part < 0 ? (int)all : (int)(all * (unit.part + 1) / a.ksplit);
 
   bf16x8 kf[KB][NS], vf[KB][NS];
   f32x4 dk[ND][KB], dv[ND][KB];
@@ -650,9 +752,10 @@ __global__ __launch_bounds__(64 * DkvShape<D>::kW) __attribute__((amdgpu_waves_p
     const int a4 = lane & 3, j4 = (lane & 15) >> 2;
     const uint32_t ta = lds0 + (4 * kg + j4) * (2 * D) + (((a4 >> 1) ^ sw16<D>(4 * kg + j4)) << 4) + (a4 & 1) * 8;
 
-    auto step = [&](uint32_t base, int slot2, int first) {
-      ring_wait<2 * Dma::kDI + 1>();
-      dma(slot2);
+    auto step = [&](uint32_t base, int slot2, int first, bool last) {
+      ring_wait<BUFS == 3 ? 2 * Dma::kDI + 1 : 0>();
+      if (BUFS == 3 || !last) dma(slot2);
+      if (k0 >= nkb || (CAUSAL && first >= kGT)) return;  // no key here, or none that the tile's queries see
       auto half = [&](auto j_c) {  // queries 32 j .. + 31 of the tile
         constexpr int J = decltype(j_c)::value, OFF = 32 * 2 * D * J;
         uint32_t pp[KB][4], ds[KB][4];  // P and dS, B operands: key block i
@@ -775,15 +878,16 @@ __global__ __launch_bounds__(64 * DkvShape<D>::kW) __attribute__((amdgpu_waves_p
     };
     int t = t0 + s0 % per;  // this step's query tile
     dma(0);
-    dma(1);
+    if (BUFS == 3) dma(1);
     int slot = 0;
     for (int st = s0; st < s1; ++st) {
       // causal: key k is hidden from query q where k - shift > q; `first` is
       // that of this wave's first key against the tile's first query
       const int64_t first = k0 - shift - (int64_t)t * kGT;
-      step(slot * kPair, slot == 0 ? 2 : slot - 1, (int)max(min(first, (int64_t)2 * kGT), (int64_t)-2 * kGT));
+      step(slot * kPair, slot == 0 ? BUFS - 1 : slot - 1, (int)max(min(first, (int64_t)2 * kGT), (int64_t)-2 * kGT),
+           st + 1 == s1);
       if (++t == nqt) t = t0;
-      slot = slot == 2 ? 0 : slot + 1;
+      slot = slot == BUFS - 1 ? 0 : slot + 1;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
@@ -793,14 +897,13 @@ __global__ __launch_bounds__(64 * DkvShape<D>::kW) __attribute__((amdgpu_waves_p
     const int64_t ki = k0 + 16 * i + c16;
     if (ki >= a.nk) continue;
     const bool live = ki < nkb;
-    if (a.splits > 1) {
-      const int64_t all_keys = a.batch * a.kv_heads * a.nk * D;
-      float* o = a.part + (int64_t)part * 2 * all_keys + (bh * a.nk + ki) * D + 4 * kg;
+    if (unit.part >= 0) {
+      float* o = a.part + ((int64_t)(blockIdx.x - a.nfull) * kKeys + wv * 32 + 16 * i + c16) * 2 * D + 4 * kg;
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
         *(f32x4*)(o + 16 * d) = live ? dk[d][i] * a.scale : zero;
-        *(f32x4*)(o + all_keys + 16 * d) = live ? dv[d][i] : zero;
+        *(f32x4*)(o + D + 16 * d) = live ? dv[d][i] : zero;
       }
       continue;
     }
@@ -816,47 +919,121 @@ __global__ __launch_bounds__(64 * DkvShape<D>::kW) __attribute__((amdgpu_waves_p
   }
 }
 
-// dk and dv from their parts, in part order; 8 values a thread.
+// The gradients of the blocks that ran in parts, added in part order; 8 values
+// a thread. Side 0: dq (rows of D), side 1: dk and dv (rows of 2 D).
+struct GradJoin {
+  const float* part;
+  uint16_t *o, *o2;
+  int64_t s[3], s2[3];
+  int64_t nfull, n;  // blocks run whole, rows of the tensor
+  int ksplit, blocks, rows, heads, causal;
+  int64_t units;     // threads
+};
+struct GradJoins {
+  GradJoin side[2];
+  int64_t blocks0;   // workgroups of side 0
+};
 template <int D>
-__global__ __launch_bounds__(256) void k_attn_dkv_join(AttnGradArgs a) {
-  const int64_t all = a.batch * a.kv_heads * a.nk * D;
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
-  if (i >= 2 * all) return;
-  const bool second = i >= all;
-  const int64_t e = second ? i - all : i;
+__global__ __launch_bounds__(256) void k_attn_grad_join(GradJoins a) {
+  const bool second = (int64_t)blockIdx.x >= a.blocks0;
+  const GradJoin& j = second ? a.side[1] : a.side[0];
+  const int64_t i = ((int64_t)blockIdx.x - (second ? a.blocks0 : 0)) * 256 + threadIdx.x;
+  if (i >= j.units) return;
+  const int width = second ? 2 * D : D;
+  const int64_t r = i / (width / 8);
+  int c = 8 * (int)(i - r * (width / 8));
+  const int64_t blk = r / j.rows, wg = j.nfull + blk, row = r - blk * j.rows;
+  int b8 = (int)(wg % j.blocks);
+  if (j.causal) b8 = j.blocks - 1 - b8;
+  const int64_t at = (int64_t)b8 * j.rows + row;
+  if (at >= j.n) return;
+  const int64_t bh = wg / j.blocks, b = bh / j.heads, h = bh - b * j.heads;
+  const float* f = j.part + (blk * j.ksplit * j.rows + row) * width + c;
   float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int p = 0; p < a.splits; ++p) {
-    const float* f = a.part + (int64_t)p * 2 * all + i;
+  for (int p = 0; p < j.ksplit; ++p, f += (int64_t)j.rows * width) {
     const float4 u = *(const float4*)f, v = *(const float4*)(f + 4);
     s[0] += u.x, s[1] += u.y, s[2] += u.z, s[3] += u.w, s[4] += v.x, s[5] += v.y, s[6] += v.z, s[7] += v.w;
   }
-  const int64_t row = e / D;  // (b, hk, key)
-  const int64_t bh = row / a.nk, key = row - bh * a.nk;
-  const int64_t b = bh / a.kv_heads, hk = bh - b * a.kv_heads;
-  uint16_t* o = second ? a.dv + b * a.dv_s[0] + key * a.dv_s[1] + hk * a.dv_s[2]
-                       : a.dk + b * a.dk_s[0] + key * a.dk_s[1] + hk * a.dk_s[2];
-  *(uint4*)(o + e % D) = pack8(s);
+  const bool two = c >= D;
+  if (two) c -= D;
+  uint16_t* o = two ? j.o2 + b * j.s2[0] + at * j.s2[1] + h * j.s2[2] : j.o + b * j.s[0] + at * j.s[1] + h * j.s[2];
+  *(uint4*)(o + c) = pack8(s);
 }
 
 // -------------------------------------------------------------------- host
 static int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
-// Parts of a key block's query steps: as many as bring the launch to two
-// workgroups a CU, each of at least four steps.
-static int dkv_splits(int64_t batch, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads) {
-  const int64_t wgs = batch * kv_heads * ((nk + 255) / 256);
-  const int64_t steps = (nq + kGT - 1) / kGT * (heads / kv_heads);
-  const int64_t want = 2 * (int64_t)cu_count() / wgs;
-  return (int)max((int64_t)1, min(min(want, steps / 4), (int64_t)16));
+// Which of a kernel's blocks run whole, and the parts of the others.
+struct GradPlan {
+  int64_t blocks, nfull;
+  int ksplit;
+  int64_t units() const { return nfull + (blocks - nfull) * ksplit; }
+  int64_t parts() const { return units() - nfull; }
+};
+// `blocks` blocks of `steps` steps each (step_us) run `slots` at a time.
+// Candidates: all whole; the last, partial round (the only one) in k parts.
+// A part costs its own start (fixed_us) and part_bytes written and read back
+// by a join.
+static GradPlan grad_plan(int64_t blocks, int64_t steps, int64_t slots, double step_us, double part_bytes) {
+  const double fixed_us = 4.0, join_us = 4.0, bytes_per_us = 4e6;
+  GradPlan best = {blocks, blocks, 1};
+  const int64_t whole = blocks / slots * slots, rest = blocks - whole;
+  if (!rest || steps < 2) return best;
+  double least = steps * step_us;  // of the last round
+  for (int k = 2; k <= 16 && k <= steps; ++k) {
+    const int64_t rounds = (rest * k + slots - 1) / slots;
+    const double us = rounds * ((double)((steps + k - 1) / k) * step_us + fixed_us) - fixed_us + join_us +
+                      2.0 * rest * k * part_bytes / bytes_per_us;
+    if (us < least) least = us, best = {blocks, whole, k};
+  }
+  return best;
 }
 
-static bool grad_strides(const void* p, const int64_t* s, int64_t tokens) {
+// The forms of the three kernels: many steps run 8 waves and three tile pairs
+// in one workgroup per CU (D 128); few, or few rows, 4 waves and two pairs in
+// two, one's loads and stores under the other's products.
+static bool few_steps(int64_t own_rows, int64_t other_rows) { return other_rows <= 16 * kGT || own_rows <= 128; }
+static int grad_waves(int64_t head_dim, bool few) { return head_dim == 64 || few ? 4 : 8; }
+static int64_t grad_slots(int64_t head_dim, bool few, int per_cu64) {
+  return (int64_t)cu_count() * (head_dim == 64 ? per_cu64 : few ? 2 : 1);
+}
+
+static GradPlan rows_plan(const AttnGradArgs& a, int64_t d, bool dq) {
+  const bool few = few_steps(a.nq, a.nk);
+  const int rows = 32 * grad_waves(d, few);
+  const int64_t blocks = a.batch * a.heads * ((a.nq + rows - 1) / rows);
+  const double step = (dq ? 2.6 : 1.8) * (d == 64 || few ? 0.6 : 1.0);
+  // causal blocks differ in length: they fill the last round by themselves
+  const int64_t slots = grad_slots(d, few, 3);
+  if (a.causal && blocks >= slots) return {blocks, blocks, 1};
+  return grad_plan(blocks, (a.nk + kGT - 1) / kGT, slots, step, rows * (d + (dq ? 0 : 2)) * 4.0);
+}
+// (k_attn_dkv's causal 4-wave form would not fit its registers.)
+static bool few_query_steps(const AttnGradArgs& a) { return !a.causal && few_steps(a.nk, a.nq * a.group); }
+static GradPlan keys_plan(const AttnGradArgs& a, int64_t d) {
+  const bool few = few_query_steps(a);
+  const int rows = 32 * grad_waves(d, few);
+  const int64_t blocks = a.batch * a.kv_heads * ((a.nk + rows - 1) / rows);
+  const int64_t slots = grad_slots(d, few, 3);
+  if (a.causal && blocks >= slots) return {blocks, blocks, 1};
+  return grad_plan(blocks, (a.nq + kGT - 1) / kGT * a.group, slots, 3.5 * (d == 64 || few ? 0.6 : 1.0),
+                   rows * d * 8.0);
+}
+
+// The offsets of a tile's rows are 32-bit; with one query a sequence, the
+// heads are its rows.
+static bool grad_strides(const void* p, const int64_t* s, int64_t tokens, bool heads_are_rows = false) {
   if (!p || !aligned(p, 16)) return false;
   for (int i = 0; i < 3; ++i)
     if (s[i] % 8) return false;
-  return tokens <= 1 || (s[1] >= 0 && s[1] < (1 << 24));  // a tile's offsets are 32-bit
+  if (heads_are_rows && (s[2] < 0 || s[2] >= (1 << 24))) return false;
+  return tokens <= 1 || (s[1] >= 0 && s[1] < (1 << 24));
 }
 
+static void gset3(int64_t* d, const int64_t* s) { d[0] = s[0], d[1] = s[1], d[2] = s[2]; }
+
+// Shape checks; a single query per sequence sees every valid key, causal or
+// not, so the query heads of a key head become the queries of one.
 static int grad_shape(AttnGradArgs& a, int64_t batch, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads,
                       int64_t head_dim, float scale, int causal, const int32_t* k_lens) {
   if (head_dim != 64 && head_dim != 128) return unsupported("head_dim %lld", (long long)head_dim);
@@ -865,7 +1042,7 @@ static int grad_shape(AttnGradArgs& a, int64_t batch, int64_t nq, int64_t nk, in
                 (long long)heads, (long long)kv_heads);
   if (nq > (1 << 30) || nk > (1 << 30) || heads > (1 << 20) || batch > (1 << 20))
     return unsupported("shape (%lld, %lld, %lld, %lld)", (long long)batch, (long long)nq, (long long)nk, (long long)heads);
-  if (batch * heads * ((nq + 31) / 32) > INT32_MAX || batch * kv_heads * ((nk + 31) / 32) > INT32_MAX / 16)
+  if (batch * heads * ((nq + 31) / 32) > INT32_MAX / 16 || batch * kv_heads * ((nk + 31) / 32) > INT32_MAX / 16)
     return unsupported("more than 2^31 workgroups");
   if ((nq + kGT - 1) / kGT * (heads / kv_heads) > INT32_MAX / 64) return unsupported("too many queries per key head");
   if (!(scale > 0.0f) || scale > 1e30f) return fail("softmax scale");
@@ -875,75 +1052,155 @@ static int grad_shape(AttnGradArgs& a, int64_t batch, int64_t nq, int64_t nk, in
   a.scale = scale, a.scale_log2 = scale * kLog2e;
   a.causal = causal ? 1 : 0;
   a.k_lens = k_lens;
+  if (nq == 1) {
+    a.nq = a.group, a.heads = a.kv_heads, a.group = 1;
+    a.causal = 0;
+  }
   return OGA_OK;
 }
-
-template <int D, int W>
-static void lse_launch(AttnGradArgs& a, hipStream_t s) {
-  a.blocks = (int)((a.nq + 32 * W - 1) / (32 * W));
-  const dim3 grid((unsigned)(a.batch * a.heads * a.blocks)), block(64 * W);
-  if (a.causal)
-    k_attn_lse<D, W, true><<<grid, block, 0, s>>>(a);
-  else
-    k_attn_lse<D, W, false><<<grid, block, 0, s>>>(a);
+// Strides of q, o, dout or dq under that view.
+static void query_strides(const AttnGradArgs& a, bool one_query, int64_t* d, const int64_t* s) {
+  gset3(d, s);
+  if (one_query) d[1] = s[2], d[2] = s[2] * a.nq;  // (a.nq: the group)
 }
 
-template <int D>
-static void bwd_launch(AttnGradArgs& a, hipStream_t s) {
-  const int64_t nqp = (a.nq + kGT - 1) / kGT * kGT;
-  const int per = 256 / (D / 8);
-  k_attn_delta<D><<<dim3((unsigned)((a.batch * nqp * a.heads + per - 1) / per)), dim3(256), 0, s>>>(a);
-  const dim3 block(64 * kGW);
-  a.blocks = (int)((a.nq + 32 * kGW - 1) / (32 * kGW));
-  const dim3 gq((unsigned)(a.batch * a.heads * a.blocks));
+// Workspaces: forward [parts of O | m, l]; backward [lse2 and Delta | parts of
+// dq | parts of dk and dv].
+struct GradSpace {
+  GradPlan rows, keys;
+  int64_t ml, dq, dkv, total;
+};
+static GradSpace fwd_space(const AttnGradArgs& a, int64_t d) {
+  GradSpace w = {};
+  w.rows = rows_plan(a, d, false);
+  const int64_t rows = w.rows.parts() * 32 * grad_waves(d, few_steps(a.nq, a.nk));
+  w.ml = align256(rows * d * 4);
+  w.total = rows ? w.ml + align256(rows * 8) : 0;
+  return w;
+}
+static GradSpace bwd_space(const AttnGradArgs& a, int64_t d) {
+  GradSpace w = {};
+  w.rows = rows_plan(a, d, true);
+  w.keys = keys_plan(a, d);
+  w.dq = align256(a.batch * a.heads * ((a.nq + kGT - 1) / kGT) * 128 * 4);
+  w.dkv = w.dq + align256(w.rows.parts() * 32 * grad_waves(d, few_steps(a.nq, a.nk)) * d * 4);
+  w.total = w.dkv + align256(w.keys.parts() * 32 * grad_waves(d, few_query_steps(a)) * d * 8);
+  return w;
+}
+
+template <int D, int W, int BUFS>
+static void lse_launch(AttnGradArgs& a, const GradPlan& p, hipStream_t s) {
+  a.blocks = (int)((a.nq + 32 * W - 1) / (32 * W));
+  a.nfull = p.nfull, a.ksplit = p.ksplit;
+  const dim3 grid((unsigned)p.units()), block(64 * W);
   if (a.causal)
-    k_attn_dq<D, true><<<gq, block, 0, s>>>(a);
+    k_attn_lse<D, W, BUFS, true><<<grid, block, 0, s>>>(a);
   else
-    k_attn_dq<D, false><<<gq, block, 0, s>>>(a);
-  a.blocks = (int)((a.nk + DkvShape<D>::kKeys - 1) / DkvShape<D>::kKeys);
-  const dim3 gk((unsigned)(a.batch * a.kv_heads * a.blocks * a.splits)), bk(64 * DkvShape<D>::kW);
-  if (a.causal)
-    k_attn_dkv<D, true><<<gk, bk, 0, s>>>(a);
-  else
-    k_attn_dkv<D, false><<<gk, bk, 0, s>>>(a);
-  if (a.splits > 1) {
-    const int64_t n = 2 * a.batch * a.kv_heads * a.nk * D / 8;
-    k_attn_dkv_join<D><<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s>>>(a);
+    k_attn_lse<D, W, BUFS, false><<<grid, block, 0, s>>>(a);
+  if (p.parts()) {
+    const int64_t rows = (p.blocks - p.nfull) * 32 * W, per = 256 / (D / 8);
+    k_attn_lse_join<D, 32 * W><<<dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, s>>>(a);
   }
 }
 
-static void gset3(int64_t* d, const int64_t* s) { d[0] = s[0], d[1] = s[1], d[2] = s[2]; }
+template <int D, int W, int BUFS>
+static GradJoin dq_launch(AttnGradArgs a, const GradPlan& p, hipStream_t s) {
+  a.blocks = (int)((a.nq + 32 * W - 1) / (32 * W));
+  a.nfull = p.nfull, a.ksplit = p.ksplit;
+  const dim3 grid((unsigned)p.units()), block(64 * W);
+  if (a.causal)
+    k_attn_dq<D, W, BUFS, true><<<grid, block, 0, s>>>(a);
+  else
+    k_attn_dq<D, W, BUFS, false><<<grid, block, 0, s>>>(a);
+  GradJoin j = {a.part, a.dq, nullptr, {}, {}, p.nfull, a.nq, p.ksplit, a.blocks, 32 * W, a.heads, a.causal,
+                (p.blocks - p.nfull) * 32 * W * (D / 8)};
+  gset3(j.s, a.dq_s);
+  return j;
+}
+
+template <int D, int W, int BUFS>
+static GradJoin dkv_launch(AttnGradArgs a, const GradPlan& p, hipStream_t s) {
+  a.blocks = (int)((a.nk + 32 * W - 1) / (32 * W));
+  a.nfull = p.nfull, a.ksplit = p.ksplit;
+  const dim3 grid((unsigned)p.units()), block(64 * W);
+  if (a.causal) {
+    if constexpr (D == 64 || W == 8) k_attn_dkv<D, W, BUFS, true><<<grid, block, 0, s>>>(a);
+  } else
+    k_attn_dkv<D, W, BUFS, false><<<grid, block, 0, s>>>(a);
+  GradJoin j = {a.part, a.dk, a.dv, {}, {}, p.nfull, a.nk, p.ksplit, a.blocks, 32 * W, a.kv_heads, 0,
+                (p.blocks - p.nfull) * 32 * W * (2 * D / 8)};
+  gset3(j.s, a.dk_s), gset3(j.s2, a.dv_s);
+  return j;
+}
+
+template <int D>
+static void bwd_launch(AttnGradArgs& a, const GradSpace& w, char* ws, hipStream_t s) {
+  a.ld = (float*)ws;
+  const int64_t nqp = (a.nq + kGT - 1) / kGT * kGT;
+  const int per = 256 / (D / 8);
+  k_attn_delta<D><<<dim3((unsigned)((a.batch * nqp * a.heads + per - 1) / per)), dim3(256), 0, s>>>(a);
+  const bool few_q = few_steps(a.nq, a.nk), few_k = few_query_steps(a);
+  GradJoins j = {};
+  a.part = (float*)(ws + w.dq);
+  if constexpr (D == 64) {
+    j.side[0] = dq_launch<D, 4, 3>(a, w.rows, s);
+  } else {
+    j.side[0] = few_q ? dq_launch<D, 4, 2>(a, w.rows, s) : dq_launch<D, 8, 3>(a, w.rows, s);
+  }
+  a.part = (float*)(ws + w.dkv);
+  if constexpr (D == 64) {
+    j.side[1] = dkv_launch<D, 4, 3>(a, w.keys, s);
+  } else {
+    j.side[1] = few_k ? dkv_launch<D, 4, 2>(a, w.keys, s) : dkv_launch<D, 8, 3>(a, w.keys, s);
+  }
+  j.blocks0 = (j.side[0].units + 255) / 256;
+  const int64_t grid = j.blocks0 + (j.side[1].units + 255) / 256;
+  if (grid) k_attn_grad_join<D><<<dim3((unsigned)grid), dim3(256), 0, s>>>(j);
+}
 
 }  // namespace oga
 
 using namespace oga;
 
+extern "C" int64_t oga_attention_lse_workspace_bytes(int64_t batch, int64_t nq, int64_t nk, int64_t heads,
+                                                     int64_t kv_heads, int64_t head_dim, int causal) {
+  AttnGradArgs a = {};
+  if (grad_shape(a, batch, nq, nk, heads, kv_heads, head_dim, 1.0f, causal, nullptr)) return 0;
+  return fwd_space(a, head_dim).total;
+}
+
 extern "C" int oga_attention_lse(const void* q, const int64_t q_strides[3], const void* k, const int64_t k_strides[3],
                                  const void* v, const int64_t v_strides[3], void* o, const int64_t o_strides[3],
                                  float* lse, int64_t batch, int64_t nq, int64_t nk, int64_t heads, int64_t kv_heads,
                                  int64_t head_dim, float softmax_scale, int causal, const int32_t* k_lens,
-                                 void* stream) {
+                                 void* workspace, int64_t workspace_bytes, void* stream) {
   AttnGradArgs a = {};
   if (int rc = grad_shape(a, batch, nq, nk, heads, kv_heads, head_dim, softmax_scale, causal, k_lens)) return rc;
-  if (!grad_strides(q, q_strides, nq) || !grad_strides(k, k_strides, nk) || !grad_strides(v, v_strides, nk) ||
-      !grad_strides(o, o_strides, nq) || !lse || !aligned(lse, 4))
+  if (!grad_strides(q, q_strides, nq, nq == 1) || !grad_strides(k, k_strides, nk) || !grad_strides(v, v_strides, nk) ||
+      !grad_strides(o, o_strides, nq, nq == 1) || !lse || !aligned(lse, 4))
     return fail("operand layout");
+  const GradSpace w = fwd_space(a, head_dim);
+  if (w.total && (!workspace || !aligned(workspace, 256) || workspace_bytes < w.total))
+    return fail("workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)w.total);
   a.q = (const uint16_t*)q, a.k = (const uint16_t*)k, a.v = (const uint16_t*)v, a.o = (uint16_t*)o, a.lse = lse;
-  gset3(a.q_s, q_strides), gset3(a.k_s, k_strides), gset3(a.v_s, v_strides), gset3(a.o_s, o_strides);
+  query_strides(a, nq == 1, a.q_s, q_strides), query_strides(a, nq == 1, a.o_s, o_strides);
+  gset3(a.k_s, k_strides), gset3(a.v_s, v_strides);
+  a.part = (float*)workspace, a.part_ml = (float*)((char*)workspace + w.ml);
   const hipStream_t s = (hipStream_t)stream;
-  if (head_dim == 128)
-    nq > 64 ? lse_launch<128, 8>(a, s) : lse_launch<128, 2>(a, s);
+  if (head_dim == 64)
+    lse_launch<64, 4, 3>(a, w.rows, s);
+  else if (few_steps(a.nq, a.nk))
+    lse_launch<128, 4, 2>(a, w.rows, s);
   else
-    nq > 64 ? lse_launch<64, 8>(a, s) : lse_launch<64, 2>(a, s);
+    lse_launch<128, 8, 3>(a, w.rows, s);
   return launch_status();
 }
 
 extern "C" int64_t oga_attention_bwd_workspace_bytes(int64_t batch, int64_t nq, int64_t nk, int64_t heads,
-                                                     int64_t kv_heads, int64_t head_dim) {
-  if (batch < 1 || nq < 1 || nk < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads) return 0;
-  const int64_t ld = align256(batch * heads * ((nq + kGT - 1) / kGT) * 128 * 4);
-  const int splits = dkv_splits(batch, nq, nk, heads, kv_heads);
-  return ld + (splits > 1 ? splits * 2 * batch * kv_heads * nk * head_dim * 4 : 0);
+                                                     int64_t kv_heads, int64_t head_dim, int causal) {
+  AttnGradArgs a = {};
+  if (grad_shape(a, batch, nq, nk, heads, kv_heads, head_dim, 1.0f, causal, nullptr)) return 0;
+  return bwd_space(a, head_dim).total;
 }
 
 extern "C" int oga_attention_bwd(const void* dout, const int64_t do_strides[3], const void* q,
@@ -956,25 +1213,22 @@ extern "C" int oga_attention_bwd(const void* dout, const int64_t do_strides[3], 
                                  int64_t workspace_bytes, void* stream) {
   AttnGradArgs a = {};
   if (int rc = grad_shape(a, batch, nq, nk, heads, kv_heads, head_dim, softmax_scale, causal, k_lens)) return rc;
-  if (!grad_strides(dout, do_strides, nq) || !grad_strides(q, q_strides, nq) || !grad_strides(k, k_strides, nk) ||
-      !grad_strides(v, v_strides, nk) || !grad_strides(out, o_strides, nq) || !grad_strides(dq, dq_strides, nq) ||
+  if (!grad_strides(dout, do_strides, nq, nq == 1) || !grad_strides(q, q_strides, nq, nq == 1) || !grad_strides(k, k_strides, nk) ||
+      !grad_strides(v, v_strides, nk) || !grad_strides(out, o_strides, nq, nq == 1) || !grad_strides(dq, dq_strides, nq, nq == 1) ||
       !grad_strides(dk, dk_strides, nk) || !grad_strides(dv, dv_strides, nk) || !lse || !aligned(lse, 4))
     return fail("operand layout");
-  const int64_t need = oga_attention_bwd_workspace_bytes(batch, nq, nk, heads, kv_heads, head_dim);
-  if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
-    return fail("workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  const GradSpace w = bwd_space(a, head_dim);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < w.total)
+    return fail("workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)w.total);
   a.dout = (const uint16_t*)dout, a.q = (const uint16_t*)q, a.k = (const uint16_t*)k, a.v = (const uint16_t*)v;
   a.out = (const uint16_t*)out, a.lse = const_cast<float*>(lse);
   a.dq = (uint16_t*)dq, a.dk = (uint16_t*)dk, a.dv = (uint16_t*)dv;
-  gset3(a.do_s, do_strides), gset3(a.q_s, q_strides), gset3(a.k_s, k_strides), gset3(a.v_s, v_strides);
-  gset3(a.o_s, o_strides), gset3(a.dq_s, dq_strides), gset3(a.dk_s, dk_strides), gset3(a.dv_s, dv_strides);
-  a.ld = (float*)workspace;
-  a.splits = dkv_splits(batch, nq, nk, heads, kv_heads);
-  a.part = (float*)((char*)workspace + align256(batch * heads * ((nq + kGT - 1) / kGT) * 128 * 4));
-  const hipStream_t s = (hipStream_t)stream;
+  query_strides(a, nq == 1, a.do_s, do_strides), query_strides(a, nq == 1, a.q_s, q_strides);
+  query_strides(a, nq == 1, a.o_s, o_strides), query_strides(a, nq == 1, a.dq_s, dq_strides);
+  gset3(a.k_s, k_strides), gset3(a.v_s, v_strides), gset3(a.dk_s, dk_strides), gset3(a.dv_s, dv_strides);
   if (head_dim == 128)
-    bwd_launch<128>(a, s);
+    bwd_launch<128>(a, w, (char*)workspace, (hipStream_t)stream);
   else
-    bwd_launch<64>(a, s);
+    bwd_launch<64>(a, w, (char*)workspace, (hipStream_t)stream);
   return launch_status();
 }

@@ -144,6 +144,7 @@ PyMethodDef kMethods[] = {
     OGA_FN(oga_fp8_dequant_per_head),
     OGA_FN(oga_attention_fp8_workspace_bytes),
     OGA_FN(oga_attention_fp8_ws),
+    OGA_FN(oga_attention_lse_workspace_bytes),
     OGA_FN(oga_attention_lse),
     OGA_FN(oga_attention_bwd_workspace_bytes),
     OGA_FN(oga_attention_bwd),

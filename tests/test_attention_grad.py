@@ -166,9 +166,10 @@ def test_entry_points_refuse_what_the_kernels_do_not_take():
     lib = _lib.load()
     st, p = _lib.strides((8192, 128, 128)), 4096
 
-    def lse(q=p, qs=st, batch=1, nq=4, nk=4, heads=1, kv_heads=1, dim=128, scale=0.1):
+    def lse(q=p, qs=st, batch=1, nq=4, nk=4, heads=1, kv_heads=1, dim=128, scale=0.1,
+            ws=None, size=0):
         return lib.oga_attention_lse(q, qs, p, st, p, st, p, st, p, batch, nq, nk, heads, kv_heads, dim, scale, 0,
-                                     None, None)
+                                     None, ws, size, None)
 
     assert lse(dim=96) == -2 and lse(dim=32) == -2
     for kw in ({"q": None}, {"q": 4104}, {"qs": _lib.strides((8192, 4, 128))}, {"qs": _lib.strides((0, 1 << 24, 8))},
@@ -176,8 +177,13 @@ def test_entry_points_refuse_what_the_kernels_do_not_take():
                {"scale": float("nan")}, {"scale": float("inf")}):
         assert lse(**kw) == -1, kw
     assert lse(nq=1 << 31) == -2 and lse(batch=1 << 20, heads=1 << 20) == -2
-    need = lib.oga_attention_bwd_workspace_bytes(1, 4, 4, 1, 1, 128)
-    assert need >= 512 and lib.oga_attention_bwd_workspace_bytes(1, 4, 4, 3, 2, 128) == 0
+    need = lib.oga_attention_lse_workspace_bytes(1, 4, 4096, 1, 1, 128, 0)
+    assert need > 0  # one block, cut over its keys
+    for kw in ({}, {"ws": p, "size": need - 1}, {"ws": p + 16, "size": need}):
+        assert lse(nk=4096, **kw) == -1 and b"workspace" in lib.oga_last_error()
+    assert lse(nq=1, heads=4, qs=_lib.strides((0, 0, 1 << 24))) == -1  # one query: heads are its rows
+    need = lib.oga_attention_bwd_workspace_bytes(1, 4, 4, 1, 1, 128, 0)
+    assert need >= 512 and lib.oga_attention_bwd_workspace_bytes(1, 4, 4, 3, 2, 128, 0) == 0
 
     def bwd(ws, size):
         return lib.oga_attention_bwd(p, st, p, st, p, st, p, st, p, st, p, p, st, p, st, p, st, 1, 4, 4, 1, 1, 128,
