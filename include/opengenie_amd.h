@@ -527,14 +527,17 @@ int oga_head_rmsnorm_rope_bwd(int x_dtype, const void* dq_out, const int64_t dqo
  * one outside 0 .. adapters - 1 is none):
  *   out = y + scale b (a x),
  * and out = y in rows without an adapter and outside all segments. low
- * [rows, rank] float32 receives scale (a x) of the rows with an adapter; the
- * backward pass reads it. Starts that do not rise give some rows an undefined
- * result, within the tensors. Rounded once, at the end.
+ * (NULL: not kept) [rows, rank] float32, 16-byte aligned, receives scale (a x)
+ * of the rows with an adapter; the backward pass reads it. Starts that do not
+ * rise give some rows an undefined result, within the tensors. Rounded once,
+ * at the end. Workspace (256-byte aligned) of oga_lora_add_workspace_bytes(...)
+ * bytes on the current device.
  */
+int64_t oga_lora_add_workspace_bytes(int64_t rows, int64_t k, int64_t rank, int64_t segments);
 int oga_lora_add(int x_dtype, const void* y, int64_t y_stride, const void* x, int64_t x_stride, const void* a,
                  const void* b, const float* scale, const int32_t* segment_starts, const int32_t* segment_adapters,
                  int64_t segments, int64_t adapters, float* low, void* out, int64_t out_stride, int64_t rows,
-                 int64_t k, int64_t n, int64_t rank, void* stream);
+                 int64_t k, int64_t n, int64_t rank, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Backward pass of oga_lora_add (y's gradient is dy itself): dx [rows, k] =
@@ -543,7 +546,8 @@ int oga_lora_add(int x_dtype, const void* y, int64_t y_stride, const void* x, in
  * an adapter without rows). Workspace (256-byte aligned) of
  * oga_lora_bwd_workspace_bytes(...) bytes on the current device.
  */
-int64_t oga_lora_bwd_workspace_bytes(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters);
+int64_t oga_lora_bwd_workspace_bytes(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters,
+                                     int64_t segments);
 int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* low,
                  const void* a, const void* b, const float* scale, const int32_t* segment_starts,
                  const int32_t* segment_adapters, int64_t segments, int64_t adapters, void* dx, int64_t dx_stride,

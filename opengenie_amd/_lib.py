@@ -114,9 +114,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "oga_head_rmsnorm_rope_bwd": (_i32, [_i32, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _p, _i32, _p, _p, _i32,
                                          _i64, _i64, _p, _i32, _i64p, _p, _i64p, _p, _i64p, _p, _p, _i64, _i64, _i64,
                                          _i64, _i64, _i64, _i32, _f32, _p, _i64, _p]),
+    "oga_lora_add_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "oga_lora_add": (_i32, [_i32, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64,
-                            _i64, _p]),
-    "oga_lora_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+                            _i64, _p, _i64, _p]),
+    "oga_lora_bwd_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64]),
     "oga_lora_bwd": (_i32, [_i32, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _p, _i64, _p, _p, _i64, _i64,
                             _i64, _i64, _p, _i64, _p]),
 }

@@ -59,17 +59,40 @@ OGA_DEVICE int64_t xcd_order(uint32_t block, uint32_t grid) {
   return (int64_t)xcd * per + min(xcd, extra) + (block >> 3);
 }
 
-// The block a workgroup works on: blocks 0 .. nfull - 1 whole, later ones in
-// ksplit parts (part -1: whole). Blocks that would fill only part of a last
-// round of the CUs (or of the only one) are cut, and a join adds the parts up.
+// The block a workgroup works on, and its part (-1: whole). Either all blocks
+// run in ksplit parts (nfull 0), or blocks 0 .. nfull - 1 whole and the rest,
+// which would fill only part of a last round of the CUs, in parts; a join adds
+// the parts up. Causal blocks differ in length: the blocks with the most steps
+// (blk 0) of all of an XCD's heads go first, so that the short ones fill up
+// the end (heads in turn, 4099 x 32 heads x 64: 143 against 157 us for dq).
 struct GradUnit {
-  int64_t wg;
-  int part;
+  int64_t bh;
+  int blk, part;
+  int64_t slot;  // of a part's place in the workspace
 };
-OGA_DEVICE GradUnit grad_unit(const AttnGradArgs& a) {
-  if ((int64_t)blockIdx.x < a.nfull) return {xcd_order(blockIdx.x, (uint32_t)a.nfull), -1};
-  const uint32_t u = blockIdx.x - (uint32_t)a.nfull;
-  return {a.nfull + u / (uint32_t)a.ksplit, (int)(u % (uint32_t)a.ksplit)};
+template <bool CAUSAL>
+OGA_DEVICE GradUnit grad_unit(const AttnGradArgs& a, int64_t bhs) {
+  const uint32_t id = blockIdx.x;
+  const int64_t nfull = a.nfull;
+  GradUnit u;
+  u.slot = 0;
+  if (nfull && id >= nfull) {
+    const uint32_t i = id - (uint32_t)nfull;
+    const int64_t wg = nfull + i / (uint32_t)a.ksplit;
+    u = {wg / a.blocks, (int)(wg % a.blocks), (int)(i % (uint32_t)a.ksplit), i};
+    return u;
+  }
+  const uint32_t kk = nfull ? 1 : a.ksplit, all = nfull ? (uint32_t)nfull : gridDim.x;
+  if (CAUSAL && bhs % 8 == 0 && all == gridDim.x) {
+    const uint32_t per = (uint32_t)(bhs / 8) * kk, w = id >> 3, r = w % per;
+    u = {(int64_t)(id & 7) * (bhs / 8) + r / kk, (int)(w / per), (int)(r % kk), 0};
+  } else {
+    const uint32_t o = (uint32_t)xcd_order(id, all), wg = o / kk;
+    u = {wg / (uint32_t)a.blocks, (int)(wg % (uint32_t)a.blocks), (int)(o % kk), 0};
+  }
+  u.slot = (u.bh * a.blocks + u.blk) * kk + u.part;
+  if (nfull) u.part = -1;
+  return u;
 }
 
 // ------------------------------------------------------------- LDS tiles
@@ -209,10 +232,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
   __shared__ uint4 smem[BUFS * kPair / 16];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const GradUnit unit = grad_unit(a);
-  int qb = (int)(unit.wg % a.blocks);
-  if (CAUSAL) qb = a.blocks - 1 - qb;  // the longest first
-  const int64_t bh = unit.wg / a.blocks;
+  const GradUnit unit = grad_unit<CAUSAL>(a, a.batch * a.heads);
+  const int qb = CAUSAL ? a.blocks - 1 - unit.blk : unit.blk;
+  const int64_t bh = unit.bh;
   const int h = (int)(bh % a.heads);
   const int64_t b = bh / a.heads;
   const int hk = h / a.group;
@@ -226,6 +248,19 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
   const int st0 = unit.part < 0 ? 0 : (int)((int64_t)nsteps * unit.part / a.ksplit);
   const int st1 = unit.part < 0 ? nsteps : (int)((int64_t)nsteps * (unit.part + 1) / a.ksplit);
 
+  const uint16_t* kb = a.k + b * a.k_s[0] + (int64_t)hk * a.k_s[2];
+  const uint16_t* vb = a.v + b * a.v_s[0] + (int64_t)hk * a.v_s[2];
+  char* const lds = (char*)smem;
+  auto dma = [&](int st, int slot) {
+    const int64_t key0 = (int64_t)st * kGT;
+    const int rows = (int)min((int64_t)kGT, nkb - key0);
+    Dma::send(kb + key0 * a.k_s[1], (uint32_t)a.k_s[1], rows, lds + slot * kPair, wv, lane);
+    Dma::send(vb + key0 * a.v_s[1], (uint32_t)a.v_s[1], rows, lds + slot * kPair + kTile, wv, lane);
+  };
+  if (st1 > st0) {  // (uniform over the workgroup) in flight under the loads below
+    dma(st0, 0);
+    if (BUFS == 3) dma(min(st0 + 1, st1 - 1), 1);
+  }
   bf16x8 qf[NS];
   {
     const uint16_t* qr = a.q + b * a.q_s[0] + min(q0 + ql, a.nq - 1) * a.q_s[1] + (int64_t)h * a.q_s[2];
@@ -239,15 +274,6 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
     for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
   float m_run = -INFINITY, l_run = 0.0f;
 
-  const uint16_t* kb = a.k + b * a.k_s[0] + (int64_t)hk * a.k_s[2];
-  const uint16_t* vb = a.v + b * a.v_s[0] + (int64_t)hk * a.v_s[2];
-  char* const lds = (char*)smem;
-  auto dma = [&](int st, int slot) {
-    const int64_t key0 = (int64_t)st * kGT;
-    const int rows = (int)min((int64_t)kGT, nkb - key0);
-    Dma::send(kb + key0 * a.k_s[1], (uint32_t)a.k_s[1], rows, lds + slot * kPair, wv, lane);
-    Dma::send(vb + key0 * a.v_s[1], (uint32_t)a.v_s[1], rows, lds + slot * kPair + kTile, wv, lane);
-  };
 
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)smem;
   const uint32_t ka = lds0 + ql * (2 * D) + ((hl ^ sw32<D>(ql)) << 4);
@@ -360,9 +386,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
     pv(IC<3>{}, v1, v0);
   };
 
-  if (st1 > st0) {  // (uniform over the workgroup)
-    dma(st0, 0);
-    if (BUFS == 3) dma(min(st0 + 1, st1 - 1), 1);
+  {
     for (int st = st0; st < st1; st += BUFS) {
       step(IC<0>{}, st);
       if (st + 1 < st1) step(IC<1>{}, st + 1);
@@ -374,7 +398,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
 
   const float l = sum_halves(l_run);
   if (unit.part >= 0) {  // O^T unnormalized, with m and l (every wave takes this branch)
-    const int64_t row = (int64_t)(blockIdx.x - a.nfull) * 32 * W + wv * 32 + ql;
+    const int64_t row = unit.slot * 32 * W + wv * 32 + ql;
+    if (q0 + ql >= a.nq) return;
     float* po = a.part + row * D;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -429,18 +454,28 @@ __global__ __launch_bounds__(256) void k_attn_lse_join(AttnGradArgs a) {
   const int c = threadIdx.x % kLpr;
   const int64_t first = blk * a.ksplit * ROWS + row;
   float m = -INFINITY;
+#pragma unroll 4
   for (int p = 0; p < a.ksplit; ++p) m = __builtin_fmaxf(m, a.part_ml[2 * (first + p * ROWS)]);
   const float nm = m == -INFINITY ? 0.0f : -m;
   float l = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int p = 0; p < a.ksplit; ++p) {
-    const int64_t at = first + p * ROWS;
-    const float2 ml = *(const float2*)(a.part_ml + 2 * at);
-    const float w = __builtin_amdgcn_exp2f(ml.x + nm);
-    l = fmaf(w, ml.y, l);
-    const float* f = a.part + at * D + 8 * c;
-    const float4 u = *(const float4*)f, v = *(const float4*)(f + 4);
-    o[0] = fmaf(w, u.x, o[0]), o[1] = fmaf(w, u.y, o[1]), o[2] = fmaf(w, u.z, o[2]), o[3] = fmaf(w, u.w, o[3]);
-    o[4] = fmaf(w, v.x, o[4]), o[5] = fmaf(w, v.y, o[5]), o[6] = fmaf(w, v.z, o[6]), o[7] = fmaf(w, v.w, o[7]);
+  for (int p0 = 0; p0 < a.ksplit; p0 += 4) {  // four parts' loads in flight
+    float2 ml[4];
+    float4 u[4], v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t at = first + min(p0 + e, a.ksplit - 1) * ROWS;
+      const float* f = a.part + at * D + 8 * c;
+      ml[e] = *(const float2*)(a.part_ml + 2 * at);
+      u[e] = *(const float4*)f, v[e] = *(const float4*)(f + 4);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (p0 + e >= a.ksplit) break;
+      const float w = __builtin_amdgcn_exp2f(ml[e].x + nm);
+      l = fmaf(w, ml[e].y, l);
+      o[0] = fmaf(w, u[e].x, o[0]), o[1] = fmaf(w, u[e].y, o[1]), o[2] = fmaf(w, u[e].z, o[2]), o[3] = fmaf(w, u[e].w, o[3]);
+      o[4] = fmaf(w, v[e].x, o[4]), o[5] = fmaf(w, v[e].y, o[5]), o[6] = fmaf(w, v[e].z, o[6]), o[7] = fmaf(w, v[e].w, o[7]);
+    }
   }
   const float inv = l > 0.0f ? 1.0f / l : l;  // no key: 0; NaN stays
 #pragma unroll
@@ -448,38 +483,6 @@ __global__ __launch_bounds__(256) void k_attn_lse_join(AttnGradArgs a) {
   const int64_t b = bh / a.heads, h = bh - b * a.heads;
   *(uint4*)(a.o + b * a.o_s[0] + qi * a.o_s[1] + h * a.o_s[2] + 8 * c) = pack8(o);
   if (c == 0) a.lse[bh * a.nq + qi] = l == 0.0f ? -INFINITY : m * kLn2 + logf(l);
-}
-
-// --------------------------------------------------- Delta and base-2 lse
-// D / 8 lanes a row of O and dO; rows behind the last query (up to the tile's
-// 64) and rows that saw no key get lse2 = +inf, so that their P is 0.
-template <int D>
-__global__ __launch_bounds__(256) void k_attn_delta(AttnGradArgs a) {
-  constexpr int kLpr = D / 8;
-  const int64_t nqp = (a.nq + kGT - 1) / kGT * kGT;
-  const int64_t row = (int64_t)blockIdx.x * (256 / kLpr) + threadIdx.x / kLpr;  // (b, n, h), h fastest
-  if (row >= a.batch * nqp * a.heads) return;
-  const int c = threadIdx.x % kLpr;
-  const int64_t bn = row / a.heads;
-  const int h = (int)(row - bn * a.heads);
-  const int64_t b = bn / nqp, n = bn - b * nqp;
-  float delta = 0.0f, lse2 = INFINITY;
-  if (n < a.nq) {
-    float f[8], g[8];
-    unpack8(*(const uint4*)(a.out + b * a.o_s[0] + n * a.o_s[1] + (int64_t)h * a.o_s[2] + 8 * c), f);
-    unpack8(*(const uint4*)(a.dout + b * a.do_s[0] + n * a.do_s[1] + (int64_t)h * a.do_s[2] + 8 * c), g);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) delta = fmaf(f[i], g[i], delta);
-    const float l = a.lse[(b * a.heads + h) * a.nq + n];
-    lse2 = l == -INFINITY ? INFINITY : l * kLog2e;
-  }
-#pragma unroll
-  for (int m = 1; m < kLpr; m <<= 1) delta += __shfl_xor(delta, m, 64);
-  if (c == 0) {
-    float* t = a.ld + ((b * a.heads + h) * (nqp / kGT) + n / kGT) * 128 + n % kGT;
-    t[0] = lse2;
-    t[64] = delta;
-  }
 }
 
 // --------------------------------------------------------------------- dq
@@ -497,10 +500,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
   __shared__ uint4 smem[BUFS * kPair / 16];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const GradUnit unit = grad_unit(a);
-  int qb = (int)(unit.wg % a.blocks);
-  if (CAUSAL) qb = a.blocks - 1 - qb;
-  const int64_t bh = unit.wg / a.blocks;
+  const GradUnit unit = grad_unit<CAUSAL>(a, a.batch * a.heads);
+  const int qb = CAUSAL ? a.blocks - 1 - unit.blk : unit.blk;
+  const int64_t bh = unit.bh;
   const int h = (int)(bh % a.heads);
   const int64_t b = bh / a.heads;
   const int hk = h / a.group;
@@ -514,7 +516,23 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
   const int st0 = unit.part < 0 ? 0 : (int)((int64_t)nsteps * unit.part / a.ksplit);
   const int st1 = unit.part < 0 ? nsteps : (int)((int64_t)nsteps * (unit.part + 1) / a.ksplit);
 
+  const uint16_t* kb = a.k + b * a.k_s[0] + (int64_t)hk * a.k_s[2];
+  const uint16_t* vb = a.v + b * a.v_s[0] + (int64_t)hk * a.v_s[2];
+  char* const lds = (char*)smem;
+  auto dma = [&](int st, int slot) {
+    const int64_t key0 = (int64_t)st * kGT;
+    const int rows = (int)min((int64_t)kGT, nkb - key0);
+    Dma::send(kb + key0 * a.k_s[1], (uint32_t)a.k_s[1], rows, lds + slot * kPair, wv, lane);
+    Dma::send(vb + key0 * a.v_s[1], (uint32_t)a.v_s[1], rows, lds + slot * kPair + kTile, wv, lane);
+  };
+  if (st1 > st0) {  // (uniform over the workgroup) in flight under the loads below
+    dma(st0, 0);
+    if (BUFS == 3) dma(min(st0 + 1, st1 - 1), 1);
+  }
   bf16x8 qf[2][NS], gf[2][NS];  // Q and dO, B operands: query 16 i + c16, d = 32 s + 8 kg ..
+  // Base-2 lse and Delta of the lane's queries, left in ld for k_attn_dkv: a
+  // query that saw no key, and the rows behind the last query up to the
+  // tile's 64, get lse2 = +inf, so that their P is 0.
   float lse2[2], delta[2];
   const int64_t nqt = (a.nq + kGT - 1) / kGT;
 #pragma unroll
@@ -527,9 +545,26 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
       qf[i][s] = __builtin_bit_cast(bf16x8, *(const uint4*)(qr + 32 * s));
       gf[i][s] = __builtin_bit_cast(bf16x8, *(const uint4*)(gr + 32 * s));
     }
-    const float* t = a.ld + (bh * nqt + qi / kGT) * 128 + qi % kGT;
-    lse2[i] = t[0];
-    delta[i] = t[64];
+    const uint16_t* orow = a.out + b * a.o_s[0] + qi * a.o_s[1] + (int64_t)h * a.o_s[2] + 8 * kg;
+    float sum = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      float x[8], y[8];
+      unpack8(*(const uint4*)(orow + 32 * s), x);
+      unpack8(__builtin_bit_cast(uint4, gf[i][s]), y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum = fmaf(x[e], y[e], sum);
+    }
+    sum += __shfl_xor(sum, 16, 64);
+    delta[i] = sum + __shfl_xor(sum, 32, 64);
+    const float l = a.lse[bh * a.nq + qi];
+    const int64_t row = q0 + 16 * i + c16;
+    lse2[i] = l == -INFINITY || row >= a.nq ? INFINITY : l * kLog2e;
+    if (kg == 0 && row < nqt * kGT && unit.part <= 0) {
+      float* t = a.ld + (bh * nqt + row / kGT) * 128 + row % kGT;
+      t[0] = lse2[i];
+      t[64] = row < a.nq ? delta[i] : 0.0f;
+    }
   }
   f32x4 acc[ND][2];
 #pragma unroll
@@ -537,15 +572,6 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
 #pragma unroll
     for (int i = 0; i < 2; ++i) acc[d][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-  const uint16_t* kb = a.k + b * a.k_s[0] + (int64_t)hk * a.k_s[2];
-  const uint16_t* vb = a.v + b * a.v_s[0] + (int64_t)hk * a.v_s[2];
-  char* const lds = (char*)smem;
-  auto dma = [&](int st, int slot) {
-    const int64_t key0 = (int64_t)st * kGT;
-    const int rows = (int)min((int64_t)kGT, nkb - key0);
-    Dma::send(kb + key0 * a.k_s[1], (uint32_t)a.k_s[1], rows, lds + slot * kPair, wv, lane);
-    Dma::send(vb + key0 * a.v_s[1], (uint32_t)a.v_s[1], rows, lds + slot * kPair + kTile, wv, lane);
-  };
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void*)smem;
   const uint32_t ra = lds0 + c16 * (2 * D) + ((kg ^ sw16<D>(c16)) << 4);
   const int a4 = lane & 3, j4 = (lane & 15) >> 2;
@@ -636,9 +662,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
     half(IC<0>{});
     half(IC<1>{});
   };
-  if (st1 > st0) {
-    dma(st0, 0);
-    if (BUFS == 3) dma(min(st0 + 1, st1 - 1), 1);
+  {
     int slot = 0;
     for (int st = st0; st < st1; ++st) {
       step(slot * kPair, slot == 0 ? BUFS - 1 : slot - 1, st);
@@ -648,11 +672,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   // lane: query 16 i + c16, d = 16 db + 4 kg .. + 3
   if (unit.part >= 0) {
-    float* o = a.part + ((int64_t)(blockIdx.x - a.nfull) * 32 * W + wv * 32 + c16) * D + 4 * kg;
+    float* o = a.part + (unit.slot * 32 * W + wv * 32 + c16) * D + 4 * kg;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i) {
+      if (q0 + 16 * i + c16 >= a.nq) continue;
 #pragma unroll
       for (int d = 0; d < ND; ++d) *(f32x4*)(o + 16 * i * D + 16 * d) = acc[d][i] * a.scale;
+    }
     return;
   }
 #pragma unroll
@@ -682,9 +708,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
   __shared__ uint4 smem[BUFS * kPair / 16];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const GradUnit unit = grad_unit(a);
-  const int kblk = (int)(unit.wg % a.blocks);
-  const int64_t bh = unit.wg / a.blocks;
+  const GradUnit unit = grad_unit<CAUSAL>(a, a.batch * a.kv_heads);
+  const int kblk = unit.blk;
+  const int64_t bh = unit.bh;
   const int hk = (int)(bh % a.kv_heads);
   const int64_t b = bh / a.kv_heads;
   const int c16 = lane & 15, kg = lane >> 4;
@@ -898,7 +924,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
     if (ki >= a.nk) continue;
     const bool live = ki < nkb;
     if (unit.part >= 0) {
-      float* o = a.part + ((int64_t)(blockIdx.x - a.nfull) * kKeys + wv * 32 + 16 * i + c16) * 2 * D + 4 * kg;
+      float* o = a.part + (unit.slot * kKeys + wv * 32 + 16 * i + c16) * 2 * D + 4 * kg;
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
         const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -950,9 +976,20 @@ __global__ __launch_bounds__(256) void k_attn_grad_join(GradJoins a) {
   const int64_t bh = wg / j.blocks, b = bh / j.heads, h = bh - b * j.heads;
   const float* f = j.part + (blk * j.ksplit * j.rows + row) * width + c;
   float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int p = 0; p < j.ksplit; ++p, f += (int64_t)j.rows * width) {
-    const float4 u = *(const float4*)f, v = *(const float4*)(f + 4);
-    s[0] += u.x, s[1] += u.y, s[2] += u.z, s[3] += u.w, s[4] += v.x, s[5] += v.y, s[6] += v.z, s[7] += v.w;
+  const int64_t step = (int64_t)j.rows * width;
+  for (int p0 = 0; p0 < j.ksplit; p0 += 4) {  // four parts' loads in flight
+    float4 u[4], v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float* g = f + min(p0 + e, j.ksplit - 1) * step;
+      u[e] = *(const float4*)g, v[e] = *(const float4*)(g + 4);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (p0 + e >= j.ksplit) break;
+      s[0] += u[e].x, s[1] += u[e].y, s[2] += u[e].z, s[3] += u[e].w;
+      s[4] += v[e].x, s[5] += v[e].y, s[6] += v[e].z, s[7] += v[e].w;
+    }
   }
   const bool two = c >= D;
   if (two) c -= D;
@@ -970,23 +1007,32 @@ struct GradPlan {
   int64_t units() const { return nfull + (blocks - nfull) * ksplit; }
   int64_t parts() const { return units() - nfull; }
 };
-// `blocks` blocks of `steps` steps each (step_us) run `slots` at a time.
-// Candidates: all whole; the last, partial round (the only one) in k parts.
-// A part costs its own start (fixed_us) and part_bytes written and read back
-// by a join.
-static GradPlan grad_plan(int64_t blocks, int64_t steps, int64_t slots, double step_us, double part_bytes) {
+// `blocks` blocks of `steps` steps each (step_us) run `slots` at a time; with
+// `fill` < 1 (causal) a block has any number of steps up to that, this share of
+// them on average. Candidates: all whole; all in k parts; with equal blocks
+// the last, partial round in k parts. A part costs its own start (fixed_us)
+// and part_bytes written and read back by a join.
+static GradPlan grad_plan(int64_t blocks, int64_t steps, int64_t slots, double step_us, double part_bytes,
+                          double fill) {
   const double fixed_us = 4.0, join_us = 4.0, bytes_per_us = 4e6;
   GradPlan best = {blocks, blocks, 1};
-  const int64_t whole = blocks / slots * slots, rest = blocks - whole;
+  const bool equal = fill >= 1.0;
+  const int64_t whole = equal ? blocks / slots * slots : 0, rest = blocks - whole;
   if (!rest || steps < 2) return best;
-  double least = steps * step_us;  // of the last round
-  for (int k = 2; k <= 16 && k <= steps; ++k) {
-    const int64_t rounds = (rest * k + slots - 1) / slots;
-    const double us = rounds * ((double)((steps + k - 1) / k) * step_us + fixed_us) - fixed_us + join_us +
-                      2.0 * rest * k * part_bytes / bytes_per_us;
-    if (us < least) least = us, best = {blocks, whole, k};
+  double least = 1e30;
+  for (int k = 1; k <= 16 && k <= steps; ++k) {
+    const double part = (double)((steps + k - 1) / k) * step_us + (k > 1 ? fixed_us : 0.0);
+    double us = equal ? (double)((rest * k + slots - 1) / slots) * part
+                      : max(part, (double)(rest * k) / slots * (fill * part) + 0.5 * part);
+    if (k > 1) us += join_us + 2.0 * rest * k * part_bytes / bytes_per_us;
+    if (us < least) least = us, best = {blocks, k == 1 ? blocks : whole, k};
   }
   return best;
+}
+// The share of the scores that a causal mask leaves.
+static double causal_fill(const AttnGradArgs& a) {
+  if (!a.causal) return 1.0;
+  return a.nk >= a.nq ? 1.0 - 0.5 * a.nq / a.nk : 0.5 * a.nk / a.nq;
 }
 
 // The forms of the three kernels: many steps run 8 waves and three tile pairs
@@ -1003,10 +1049,8 @@ static GradPlan rows_plan(const AttnGradArgs& a, int64_t d, bool dq) {
   const int rows = 32 * grad_waves(d, few);
   const int64_t blocks = a.batch * a.heads * ((a.nq + rows - 1) / rows);
   const double step = (dq ? 2.6 : 1.8) * (d == 64 || few ? 0.6 : 1.0);
-  // causal blocks differ in length: they fill the last round by themselves
-  const int64_t slots = grad_slots(d, few, 3);
-  if (a.causal && blocks >= slots) return {blocks, blocks, 1};
-  return grad_plan(blocks, (a.nk + kGT - 1) / kGT, slots, step, rows * (d + (dq ? 0 : 2)) * 4.0);
+  return grad_plan(blocks, (a.nk + kGT - 1) / kGT, grad_slots(d, few, 3), step,
+                   min((int64_t)rows, a.nq) * (d + (dq ? 0 : 2)) * 4.0, causal_fill(a));
 }
 // (k_attn_dkv's causal 4-wave form would not fit its registers.)
 static bool few_query_steps(const AttnGradArgs& a) { return !a.causal && few_steps(a.nk, a.nq * a.group); }
@@ -1014,10 +1058,8 @@ static GradPlan keys_plan(const AttnGradArgs& a, int64_t d) {
   const bool few = few_query_steps(a);
   const int rows = 32 * grad_waves(d, few);
   const int64_t blocks = a.batch * a.kv_heads * ((a.nk + rows - 1) / rows);
-  const int64_t slots = grad_slots(d, few, 3);
-  if (a.causal && blocks >= slots) return {blocks, blocks, 1};
-  return grad_plan(blocks, (a.nq + kGT - 1) / kGT * a.group, slots, 3.5 * (d == 64 || few ? 0.6 : 1.0),
-                   rows * d * 8.0);
+  return grad_plan(blocks, (a.nq + kGT - 1) / kGT * a.group, grad_slots(d, few, 3),
+                   3.5 * (d == 64 || few ? 0.6 : 1.0), min((int64_t)rows, a.nk) * d * 8.0, causal_fill(a));
 }
 
 // The offsets of a tile's rows are 32-bit; with one query a sequence, the
@@ -1136,9 +1178,6 @@ static GradJoin dkv_launch(AttnGradArgs a, const GradPlan& p, hipStream_t s) {
 template <int D>
 static void bwd_launch(AttnGradArgs& a, const GradSpace& w, char* ws, hipStream_t s) {
   a.ld = (float*)ws;
-  const int64_t nqp = (a.nq + kGT - 1) / kGT * kGT;
-  const int per = 256 / (D / 8);
-  k_attn_delta<D><<<dim3((unsigned)((a.batch * nqp * a.heads + per - 1) / per)), dim3(256), 0, s>>>(a);
   const bool few_q = few_steps(a.nq, a.nk), few_k = few_query_steps(a);
   GradJoins j = {};
   a.part = (float*)(ws + w.dq);

@@ -7,8 +7,10 @@
 //   dA_l = sum_rows dlow x^T,  dB_l = sum_rows dy low^T,  low = s_l A_l x.
 // r is small, so every product is bound by moving x, y and dy once:
 //  * k_lora_shrink: low (or dlow) [rows, r], float32, from the long rows. The
-//    waves of a workgroup divide the long axis and add up in LDS.
-//  * k_lora_expand: the [rows, N] (or [rows, K]) result from low, added to y.
+//    waves of a workgroup divide the long axis and add up in LDS; where rows
+//    are few, several workgroups divide it too and each leaves its part.
+//  * k_lora_expand: the [rows, N] (or [rows, K]) result from low, added to y;
+//    it adds the parts of low up as it reads them, in order.
 //  * k_lora_wgrad: dA and dB, one workgroup per adapter, 512 columns and part
 //    of the adapter's rows; k_lora_join adds the parts in order.
 // The sums low and dlow stay float32 in memory and enter the matrix products
@@ -116,16 +118,16 @@ struct ShrinkArgs {
   int64_t xs;
   const void* w;  // [adapters, rank, k]
   const float* scale;
-  float* low;     // [rows, rank]
+  float* low;     // [parts][rows, rank]
   int64_t k;
   int rank;
 };
 
-constexpr int kShrinkWaves = 8;
+constexpr int kShrinkWaves = 4;
 
-// 16 TB rows x 16 RB ranks per workgroup; wave w takes an eighth of the long
-// axis. The fragments come straight from memory (each row's 64-byte pieces of
-// consecutive steps share a line).
+// 16 TB rows x 16 RB ranks per workgroup, part blockIdx.y of the long axis in
+// chunks of 64 (a 128-byte line of each row), the waves in turn. The fragments
+// come straight from memory; two chunks of loads are in flight.
 template <int XDT, int RB, int TB>
 __global__ __launch_bounds__(64 * kShrinkWaves) void k_lora_shrink(ShrinkArgs a) {
   __shared__ f32x4 red[kShrinkWaves][TB * RB][64];
@@ -137,77 +139,114 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void k_lora_shrink(ShrinkArgs a)
   const uint16_t* xr[TB];
 #pragma unroll
   for (int t = 0; t < TB; ++t)
-    xr[t] = (const uint16_t*)a.x + min(max(p.tile0 + 16 * t + c, p.lo), p.hi - 1) * a.xs;
+    xr[t] = (const uint16_t*)a.x + min(max(p.tile0 + 16 * t + c, p.lo), p.hi - 1) * a.xs + kg;
   const uint16_t* wr[RB];
 #pragma unroll
   for (int r = 0; r < RB; ++r)
-    wr[r] = (const uint16_t*)a.w + ((int64_t)p.adapter * a.rank + min(16 * r + c, a.rank - 1)) * a.k;
+    wr[r] = (const uint16_t*)a.w + ((int64_t)p.adapter * a.rank + min(16 * r + c, a.rank - 1)) * a.k + kg;
   f32x4 acc[TB][RB];
 #pragma unroll
   for (int t = 0; t < TB; ++t)
 #pragma unroll
     for (int r = 0; r < RB; ++r) acc[t][r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  const int64_t steps = (a.k + 31) / 32, whole = a.k / 32;
-  const int64_t s0 = steps * wv / kShrinkWaves, s1 = steps * (wv + 1) / kShrinkWaves;
-  auto step = [&](int64_t k0, bool in) {
-    uint4 xf[TB], wf[RB];
+  struct Chunk {
+    uint4 x[2][TB], w[2][RB];
+  };
+  const int chunks = (int)((a.k + 63) / 64), whole = (int)(a.k / 64);
+  const int c0 = (int)((int64_t)chunks * blockIdx.y / gridDim.y), c1 = (int)((int64_t)chunks * (blockIdx.y + 1) / gridDim.y);
+  auto load = [&](Chunk& f, int ch) {
+    const int k0 = 64 * ch;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int t = 0; t < TB; ++t) f.x[h][t] = *(const uint4*)(xr[t] + k0 + 32 * h);
+#pragma unroll
+      for (int r = 0; r < RB; ++r) f.w[h][r] = *(const uint4*)(wr[r] + k0 + 32 * h);
+    }
+  };
+  auto mul = [&](const Chunk& f) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int t = 0; t < TB; ++t) acc[t][r] = mfma16<XDT>(f.w[h][r], f.x[h][t], acc[t][r]);
+  };
+  const int end = min(c1, whole);
+  Chunk f0, f1;
+  int ch = c0 + wv;
+  if (ch < end) load(f0, ch);
+  for (; ch < end; ch += 2 * kShrinkWaves) {
+    const bool two = ch + kShrinkWaves < end;
+    if (two) load(f1, ch + kShrinkWaves);
+    mul(f0);
+    if (ch + 2 * kShrinkWaves < end) load(f0, ch + 2 * kShrinkWaves);
+    if (two) mul(f1);
+  }
+  if (c1 > whole && wv == (whole - c0) % kShrinkWaves) {  // the last 8 .. 56 of the axis
     const uint4 none = make_uint4(0, 0, 0, 0);
 #pragma unroll
-    for (int t = 0; t < TB; ++t) xf[t] = in ? *(const uint4*)(xr[t] + k0) : none;
+    for (int h = 0; h < 2; ++h) {
+      const bool in = 64 * whole + 32 * h + kg < a.k;
 #pragma unroll
-    for (int r = 0; r < RB; ++r) wf[r] = in ? *(const uint4*)(wr[r] + k0) : none;
+      for (int t = 0; t < TB; ++t) f0.x[h][t] = in ? *(const uint4*)(xr[t] + 64 * whole + 32 * h) : none;
 #pragma unroll
-    for (int r = 0; r < RB; ++r)
-#pragma unroll
-      for (int t = 0; t < TB; ++t) acc[t][r] = mfma16<XDT>(wf[r], xf[t], acc[t][r]);
-  };
-#pragma unroll 4
-  for (int64_t s = s0; s < min(s1, whole); ++s) step(32 * s + kg, true);
-  if (s1 > whole && s1 > s0) step(32 * whole + kg, 32 * whole + kg < a.k);
+      for (int r = 0; r < RB; ++r) f0.w[h][r] = in ? *(const uint4*)(wr[r] + 64 * whole + 32 * h) : none;
+    }
+    mul(f0);
+  }
 #pragma unroll
   for (int t = 0; t < TB; ++t)
 #pragma unroll
     for (int r = 0; r < RB; ++r) red[wv][t * RB + r][lane] = acc[t][r];
   __syncthreads();
   const float scale = a.scale ? a.scale[p.adapter] : 1.0f;
+  float* const low = a.low + blockIdx.y * a.g.rows * a.rank;
   for (int o = wv; o < TB * RB; o += kShrinkWaves) {
     f32x4 v = red[0][o][lane];
 #pragma unroll
     for (int w = 1; w < kShrinkWaves; ++w) v += red[w][o][lane];
     const int64_t row = p.tile0 + 16 * (o / RB) + c;
     const int rank = 16 * (o % RB) + 4 * (lane >> 4);
-    if (row >= p.lo && row < p.hi && rank < a.rank) *(f32x4*)(a.low + row * a.rank + rank) = v * scale;
+    if (row >= p.lo && row < p.hi && rank < a.rank) *(f32x4*)(low + row * a.rank + rank) = v * scale;
   }
 }
 
 // ------------------------------------------------------------------ expand
 struct ExpandArgs {
   Segments g;
-  const float* low;  // [rows, rank]
+  const float* low;  // [parts][rows, rank]
+  float* low_sum;    // [rows, rank], their sum, or null
   const void* w;     // [adapters, n, rank]
   const void* y;     // [rows, n] or null (zero)
   void* out;         // [rows, n]; may be y
   int64_t ys, os;    // row strides
   int64_t n;
-  int rank;
-  int groups;        // 32-column groups per wave
+  int rank, parts;
 };
 
 constexpr int kExpandWaves = 4;
 
-// 16 TB rows x 32 groups columns per wave. The features of the two MFMA row
-// blocks of a group interleave by fours (block b's row 4g + i is column
-// 8g + 4b + i), so a lane ends with 8 consecutive columns of its row.
-template <int XDT, int KS, int TB>
+#ifndef OGA_EXP_PF
+#define OGA_EXP_PF 0
+#endif
+#ifndef OGA_EXP_G
+#define OGA_EXP_G 4
+#endif
+// 16 TB rows x 32 G columns per wave. The features of the two MFMA row blocks
+// of a 32-column group interleave by fours (block b's row 4g + i is column
+// 8g + 4b + i), so a lane ends with 8 consecutive columns of its row. The two
+// halves of the tile's low, which all waves use, go through LDS as fragments.
+template <int XDT, int KS, int TB, int G>
 __global__ __launch_bounds__(64 * kExpandWaves) void k_lora_expand(ExpandArgs a) {
+  __shared__ uint4 lows[TB][KS][2][64];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const Pair p = seg_pair<16 * TB>(a.g, blockIdx.x, lane);
   if (p.hi <= p.lo) return;
   const int c = lane & 15, kg = 8 * (lane >> 4);
-  const int64_t f_begin = ((int64_t)blockIdx.y * kExpandWaves + wv) * 32 * a.groups;
-  const int64_t f_end = min(f_begin + 32 * a.groups, a.n);
-  if (f_begin >= f_end) return;
+  const int64_t f_begin = ((int64_t)blockIdx.y * kExpandWaves + wv) * 32 * G;
+  const int64_t f_end = min(f_begin + 32 * G, a.n);
   if (p.adapter < 0) {  // rows without an adapter keep y (dx: zero)
     if (a.y == a.out) return;
     for (int64_t f = f_begin + kg; f < f_end; f += 32)
@@ -221,56 +260,96 @@ __global__ __launch_bounds__(64 * kExpandWaves) void k_lora_expand(ExpandArgs a)
       }
     return;
   }
-  uint4 hi[TB][KS], lo[TB][KS];
+  // wave w takes fragments w, w + 4, ... of the tile's TB x KS
+  for (int u = wv; u < TB * KS; u += kExpandWaves) {
+    const int t = u / KS, s = u % KS;
+    const int64_t row = p.tile0 + 16 * t + c, rc = min(max(row, p.lo), p.hi - 1);
+    float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (32 * s + kg < a.rank) {
+      const int64_t step = a.g.rows * a.rank;
+      const float* l = a.low + rc * a.rank + 32 * s + kg;
+      auto add = [&](const float4& x, const float4& y) {
+        f[0] += x.x, f[1] += x.y, f[2] += x.z, f[3] += x.w, f[4] += y.x, f[5] += y.y, f[6] += y.z, f[7] += y.w;
+      };
+      int q = 0;
+      for (; q + 4 <= a.parts; q += 4) {
+        float4 x[4], y[4];
 #pragma unroll
-  for (int t = 0; t < TB; ++t) {
-    const float* l = a.low + min(max(p.tile0 + 16 * t + c, p.lo), p.hi - 1) * a.rank;
+        for (int e = 0; e < 4; ++e) x[e] = *(const float4*)(l + (q + e) * step), y[e] = *(const float4*)(l + (q + e) * step + 4);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (32 * s + kg < a.rank) {
-        const float4 u = *(const float4*)(l + 32 * s + kg), v = *(const float4*)(l + 32 * s + kg + 4);
-        f[0] = u.x, f[1] = u.y, f[2] = u.z, f[3] = u.w, f[4] = v.x, f[5] = v.y, f[6] = v.z, f[7] = v.w;
+        for (int e = 0; e < 4; ++e) add(x[e], y[e]);
       }
-      split8x<XDT>(f, hi[t][s], lo[t][s]);
+      for (; q < a.parts; ++q) add(*(const float4*)(l + q * step), *(const float4*)(l + q * step + 4));
+      if (a.low_sum && row == rc && blockIdx.y == 0) {
+        float* o = a.low_sum + row * a.rank + 32 * s + kg;
+        *(float4*)o = make_float4(f[0], f[1], f[2], f[3]);
+        *(float4*)(o + 4) = make_float4(f[4], f[5], f[6], f[7]);
+      }
     }
+    uint4 hi, lo;
+    split8x<XDT>(f, hi, lo);
+    lows[t][s][0][lane] = hi;
+    lows[t][s][1][lane] = lo;
   }
+  __syncthreads();
+  struct Group {
+    uint4 y[TB], w[2][KS];
+  };
+  const uint4 none = make_uint4(0, 0, 0, 0);
   const uint16_t* w = (const uint16_t*)a.w + (int64_t)p.adapter * a.n * a.rank;
-  for (int64_t f0 = f_begin; f0 < f_end; f0 += 32) {
-    const int64_t f = f0 + kg;  // this lane's 8 columns
-    uint4 yv[TB];
+  auto load = [&](Group& g, int64_t f0) {
+    if (a.y) {
 #pragma unroll
-    for (int t = 0; t < TB; ++t) {
-      const int64_t row = min(max(p.tile0 + 16 * t + c, p.lo), p.hi - 1);
-      yv[t] = a.y && f < a.n ? *(const uint4*)((const uint16_t*)a.y + row * a.ys + f) : make_uint4(0, 0, 0, 0);
+      for (int t = 0; t < TB; ++t)
+        g.y[t] = *(const uint4*)((const uint16_t*)a.y + min(max(p.tile0 + 16 * t + c, p.lo), p.hi - 1) * a.ys +
+                                 min(f0 + kg, a.n - 8));
     }
-    f32x4 acc[2][TB];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const int64_t feat = min(f0 + 8 * (c >> 2) + 4 * b + (c & 3), a.n - 1);
-      uint4 wf[KS];
 #pragma unroll
       for (int s = 0; s < KS; ++s)
-        wf[s] = 32 * s + kg < a.rank ? *(const uint4*)(w + feat * a.rank + 32 * s + kg) : make_uint4(0, 0, 0, 0);
+        g.w[b][s] = 32 * s + kg < a.rank ? *(const uint4*)(w + feat * a.rank + 32 * s + kg) : none;
+    }
+  };
+  Group cur, nxt;
+  if (OGA_EXP_PF && f_begin < f_end) load(cur, f_begin);
+#pragma unroll 1
+  for (int64_t f0 = f_begin; f0 < f_end; f0 += 32) {
+    const int64_t f = f0 + kg;  // this lane's 8 columns
+    if (!OGA_EXP_PF)
+      load(cur, f0);
+    else if (f0 + 32 < f_end)
+      load(nxt, f0 + 32);
+    f32x4 acc[2][TB];
 #pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        acc[b][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int t = 0; t < TB; ++t) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          acc[b][t] = mfma16<XDT>(wf[s], lo[t][s], acc[b][t]);
-          acc[b][t] = mfma16<XDT>(wf[s], hi[t][s], acc[b][t]);
+      for (int b = 0; b < 2; ++b) acc[b][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int h = 1; h >= 0; --h) {
+          const uint4 l = lows[t][s][h][lane];
+#pragma unroll
+          for (int b = 0; b < 2; ++b) acc[b][t] = mfma16<XDT>(cur.w[b][s], l, acc[b][t]);
         }
-      }
     }
 #pragma unroll
     for (int t = 0; t < TB; ++t) {
       const int64_t row = p.tile0 + 16 * t + c;
       float v[8];
-      unpack8x<XDT>(yv[t], v);
+      if (a.y) {
+        unpack8x<XDT>(cur.y[t], v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = a.y ? v[i] + acc[i >> 2][t][i & 3] : acc[i >> 2][t][i & 3];
+        for (int i = 0; i < 8; ++i) v[i] += acc[i >> 2][t][i & 3];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = acc[i >> 2][t][i & 3];
+      }
       if (row >= p.lo && row < p.hi && f < a.n) *(uint4*)((uint16_t*)a.out + row * a.os + f) = pack8x<XDT>(v);
     }
+    if (OGA_EXP_PF) cur = nxt;
   }
 }
 
@@ -345,7 +424,21 @@ __global__ __launch_bounds__(256) void k_lora_wgrad(WgradArgs a) {
 #pragma unroll
     for (int r = 0; r < RB; ++r) acc[j][r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   int64_t seen = 0;  // tiles of this adapter so far
+  struct Rows8 {
+    uint4 v[8];
+  };
   auto tile = [&](int64_t lo, int64_t hi) {
+    const int steps = (int)((min(hi - lo, (int64_t)kWgradRows) + 31) / 32);
+    auto rows8 = [&](Rows8& x, int64_t first) {
+      const int64_t row = first + g8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x.v[j] = make_uint4(0, 0, 0, 0);  // rows of others may hold anything
+        if (row + j < hi) x.v[j] = *(const uint4*)((const uint16_t*)sd.x + (row + j) * sd.xs + colc);
+      }
+    };
+    Rows8 cur, nxt;
+    rows8(cur, lo);  // in flight while the tile's u goes to LDS
     __syncthreads();  // the last tile's reads are done
     const int n4 = 4 * RB;  // float4 per row
     for (int i = threadIdx.x; i < kWgradRows * n4; i += 256) {
@@ -361,15 +454,8 @@ __global__ __launch_bounds__(256) void k_lora_wgrad(WgradArgs a) {
       }
     }
     __syncthreads();
-    const int steps = (int)((min(hi - lo, (int64_t)kWgradRows) + 31) / 32);
     for (int st = 0; st < steps; ++st) {
-      const int64_t row = lo + 32 * st + g8;
-      uint4 xv[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        xv[j] = make_uint4(0, 0, 0, 0);  // rows of others may hold anything
-        if (row + j < hi) xv[j] = *(const uint4*)((const uint16_t*)sd.x + (row + j) * sd.xs + colc);
-      }
+      if (st + 1 < steps) rows8(nxt, lo + 32 * (st + 1));
       uint4 fh[RB], fl[RB];
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
@@ -381,16 +467,17 @@ __global__ __launch_bounds__(256) void k_lora_wgrad(WgradArgs a) {
       for (int j = 0; j < 8; ++j) {
         const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
         auto word = [&](const uint4& v) { return (j >> 1) == 0 ? v.x : (j >> 1) == 1 ? v.y : (j >> 1) == 2 ? v.z : v.w; };
-        const uint4 xf = make_uint4(__builtin_amdgcn_perm(word(xv[1]), word(xv[0]), sel),
-                                    __builtin_amdgcn_perm(word(xv[3]), word(xv[2]), sel),
-                                    __builtin_amdgcn_perm(word(xv[5]), word(xv[4]), sel),
-                                    __builtin_amdgcn_perm(word(xv[7]), word(xv[6]), sel));
+        const uint4 xf = make_uint4(__builtin_amdgcn_perm(word(cur.v[1]), word(cur.v[0]), sel),
+                                    __builtin_amdgcn_perm(word(cur.v[3]), word(cur.v[2]), sel),
+                                    __builtin_amdgcn_perm(word(cur.v[5]), word(cur.v[4]), sel),
+                                    __builtin_amdgcn_perm(word(cur.v[7]), word(cur.v[6]), sel));
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
           acc[j][r] = mfma16<XDT>(fl[r], xf, acc[j][r]);
           acc[j][r] = mfma16<XDT>(fh[r], xf, acc[j][r]);
         }
       }
+      cur = nxt;
     }
   };
   for (int s0 = 0; s0 < a.g.count; s0 += 64) {
@@ -455,59 +542,76 @@ __global__ __launch_bounds__(256) void k_lora_join(JoinArgs a) {
 }
 
 // -------------------------------------------------------------------- host
-// Rows of a tile: 16 where segments are short (a step's single tokens), more
-// where they are long and each fragment of the weights serves more rows.
-static bool long_segments(const Segments& g) { return g.rows >= 64 * (int64_t)g.count; }
+// Blocks of 16 rows in a tile: more where segments are long and each fragment
+// of the weights serves more rows, one where they are single tokens.
+static int row_blocks(const Segments& g, int most) {
+  const int64_t mean = g.rows / g.count;
+  return mean >= 48 ? most : mean >= 16 ? min(most, 2) : 1;
+}
+
+// Parts of the long axis: enough workgroups for four a CU, each wave with two
+// chunks or more.
+static int shrink_parts(int64_t rows, int64_t segments, int64_t k) {
+  const int64_t pairs = seg_pairs(rows, segments, rows / segments >= 16 ? 32 : 16);
+  return (int)max((int64_t)1, min(min(4 * (int64_t)cu_count() / pairs, (k + 63) / 64 / (2 * kShrinkWaves)), (int64_t)8));
+}
 
 template <int XDT, int RB>
-static void shrink_launch(const ShrinkArgs& a, hipStream_t s) {
+static void shrink_launch(const ShrinkArgs& a, int parts, hipStream_t s) {
   constexpr int TB = RB >= 8 ? 1 : 2;
-  if (long_segments(a.g))
-    k_lora_shrink<XDT, RB, TB><<<dim3((unsigned)seg_pairs(a.g.rows, a.g.count, 16 * TB)), dim3(64 * kShrinkWaves), 0, s>>>(a);
+  const dim3 block(64 * kShrinkWaves);
+  if (row_blocks(a.g, TB) == TB)
+    k_lora_shrink<XDT, RB, TB><<<dim3((unsigned)seg_pairs(a.g.rows, a.g.count, 16 * TB), parts), block, 0, s>>>(a);
   else
-    k_lora_shrink<XDT, RB, 1><<<dim3((unsigned)seg_pairs(a.g.rows, a.g.count, 16)), dim3(64 * kShrinkWaves), 0, s>>>(a);
+    k_lora_shrink<XDT, RB, 1><<<dim3((unsigned)seg_pairs(a.g.rows, a.g.count, 16), parts), block, 0, s>>>(a);
 }
 template <int XDT>
-static void shrink(const ShrinkArgs& a, hipStream_t s) {
+static void shrink(const ShrinkArgs& a, int parts, hipStream_t s) {
   if (a.rank <= 16)
-    shrink_launch<XDT, 1>(a, s);
+    shrink_launch<XDT, 1>(a, parts, s);
   else if (a.rank <= 32)
-    shrink_launch<XDT, 2>(a, s);
+    shrink_launch<XDT, 2>(a, parts, s);
   else if (a.rank <= 64)
-    shrink_launch<XDT, 4>(a, s);
+    shrink_launch<XDT, 4>(a, parts, s);
   else
-    shrink_launch<XDT, 8>(a, s);
+    shrink_launch<XDT, 8>(a, parts, s);
 }
 
+template <int XDT, int KS, int TB, int G>
+static void expand_launch(const ExpandArgs& a, hipStream_t s) {
+  constexpr int cols = 32 * G * kExpandWaves;
+  const dim3 grid((unsigned)seg_pairs(a.g.rows, a.g.count, 16 * TB), (unsigned)((a.n + cols - 1) / cols));
+  k_lora_expand<XDT, KS, TB, G><<<grid, dim3(64 * kExpandWaves), 0, s>>>(a);
+}
 template <int XDT, int KS>
-static void expand_launch(ExpandArgs a, hipStream_t s) {
-  constexpr int TB = KS >= 4 ? 2 : 4;
-  const bool wide = long_segments(a.g);
-  a.groups = wide ? 4 : 1;
-  const unsigned gy = (unsigned)((a.n + 32 * a.groups * kExpandWaves - 1) / (32 * a.groups * kExpandWaves));
-  if (wide)
-    k_lora_expand<XDT, KS, TB><<<dim3((unsigned)seg_pairs(a.g.rows, a.g.count, 16 * TB), gy), dim3(64 * kExpandWaves), 0, s>>>(a);
+static void expand_rows(const ExpandArgs& a, hipStream_t s) {
+  constexpr int most = KS >= 4 ? 2 : 4;
+  const int tb = row_blocks(a.g, most);
+  if (tb == 4)
+    expand_launch<XDT, KS, most, OGA_EXP_G>(a, s);
+  else if (tb == 2)
+    expand_launch<XDT, KS, 2, OGA_EXP_G>(a, s);
   else
-    k_lora_expand<XDT, KS, 1><<<dim3((unsigned)seg_pairs(a.g.rows, a.g.count, 16), gy), dim3(64 * kExpandWaves), 0, s>>>(a);
+    expand_launch<XDT, KS, 1, 1>(a, s);
 }
 template <int XDT>
 static void expand(const ExpandArgs& a, hipStream_t s) {
   if (a.rank <= 32)
-    expand_launch<XDT, 1>(a, s);
+    expand_rows<XDT, 1>(a, s);
   else if (a.rank <= 64)
-    expand_launch<XDT, 2>(a, s);
+    expand_rows<XDT, 2>(a, s);
   else
-    expand_launch<XDT, 4>(a, s);
+    expand_rows<XDT, 4>(a, s);
 }
 
 static int wgrad_rank_blocks(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : 4; }
 
-// Parts of each adapter's rows: enough workgroups for two a CU, but no more
+// Parts of each adapter's rows: enough workgroups for one a CU, but no more
 // than tiles of 128 rows an adapter has on average.
 static int wgrad_splits(int64_t rows, int64_t adapters, int64_t k, int64_t n, int64_t rank) {
   const int64_t rz = (rank + 16 * wgrad_rank_blocks((int)rank) - 1) / (16 * wgrad_rank_blocks((int)rank));
   const int64_t wgs = ((k + 511) / 512 + (n + 511) / 512) * adapters * rz;
-  const int64_t want = (2 * (int64_t)cu_count() + wgs - 1) / wgs;
+  const int64_t want = ((int64_t)cu_count() + wgs - 1) / wgs;
   const int64_t tiles = (rows + kWgradRows * adapters - 1) / (kWgradRows * adapters);
   return (int)max((int64_t)1, min(min(want, tiles), (int64_t)32));
 }
@@ -542,20 +646,24 @@ static bool rows_ok(const void* p, int64_t stride) { return p && aligned(p, 16) 
 
 static int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
-// Layout of the backward workspace: dlow, A^T, B^T, the partial dA and dB.
+// Layout of the backward workspace: the parts of dlow and dlow, A^T, B^T, the
+// partial dA and dB.
 struct LoraBwdSpace {
   int64_t dlow, at, bt, pa, pb, total;
-  int splits;
+  int parts, splits;
 };
-static LoraBwdSpace lora_bwd_space(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
+static LoraBwdSpace lora_bwd_space(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters,
+                                   int64_t segments) {
   LoraBwdSpace w;
+  w.parts = shrink_parts(rows, segments, n);
   w.splits = wgrad_splits(rows, adapters, k, n, rank);
-  w.dlow = 0;
-  w.at = w.dlow + align256(rows * rank * 4);
+  w.dlow = align256(w.parts * rows * rank * 4);
+  w.at = w.dlow + (w.parts > 1 ? align256(rows * rank * 4) : 0);
   w.bt = w.at + align256(adapters * rank * k * 2);
   w.pa = w.bt + align256(adapters * rank * n * 2);
   w.pb = w.pa + align256(adapters * w.splits * rank * k * 4);
   w.total = w.pb + align256(adapters * w.splits * rank * n * 4);
+  if (w.parts == 1) w.dlow = 0;
   return w;
 }
 
@@ -563,31 +671,42 @@ static LoraBwdSpace lora_bwd_space(int64_t rows, int64_t k, int64_t n, int64_t r
 
 using namespace oga;
 
+extern "C" int64_t oga_lora_add_workspace_bytes(int64_t rows, int64_t k, int64_t rank, int64_t segments) {
+  if (rows < 1 || k < 8 || rank < 8 || rank > 128 || segments < 1) return 0;
+  return align256(shrink_parts(rows, segments, k) * rows * rank * 4);
+}
+
 extern "C" int oga_lora_add(int x_dtype, const void* y, int64_t y_stride, const void* x, int64_t x_stride,
                             const void* a, const void* b, const float* scale, const int32_t* segment_starts,
                             const int32_t* segment_adapters, int64_t segments, int64_t adapters, float* low, void* out,
-                            int64_t out_stride, int64_t rows, int64_t k, int64_t n, int64_t rank, void* stream) {
+                            int64_t out_stride, int64_t rows, int64_t k, int64_t n, int64_t rank, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
   if (int rc = lora_shape(x_dtype, rows, k, n, rank, adapters, segments, segment_starts, segment_adapters)) return rc;
   if (!rows_ok(y, y_stride) || !rows_ok(x, x_stride) || !rows_ok(out, out_stride) || !rows_ok(a, k) ||
-      !rows_ok(b, rank) || !rows_ok(low, 8))
+      !rows_ok(b, rank) || !aligned(low, 16))
     return fail("operand alignment");
+  const int64_t need = oga_lora_add_workspace_bytes(rows, k, rank, segments);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
+    return fail("workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   const Segments g = {segment_starts, segment_adapters, (int)segments, (int)adapters, rows};
-  const ShrinkArgs sa = {g, x, x_stride, a, scale, low, k, (int)rank};
-  const ExpandArgs ea = {g, low, b, y, out, y_stride, out_stride, n, (int)rank, 0};
+  const int parts = shrink_parts(rows, segments, k);
+  const ShrinkArgs sa = {g, x, x_stride, a, scale, (float*)workspace, k, (int)rank};
+  const ExpandArgs ea = {g, (const float*)workspace, low, b, y, out, y_stride, out_stride, n, (int)rank, parts};
   const hipStream_t s = (hipStream_t)stream;
   if (x_dtype == OGA_DT_F16) {
-    shrink<OGA_DT_F16>(sa, s);
+    shrink<OGA_DT_F16>(sa, parts, s);
     expand<OGA_DT_F16>(ea, s);
   } else {
-    shrink<OGA_DT_BF16>(sa, s);
+    shrink<OGA_DT_BF16>(sa, parts, s);
     expand<OGA_DT_BF16>(ea, s);
   }
   return launch_status();
 }
 
-extern "C" int64_t oga_lora_bwd_workspace_bytes(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters) {
-  if (rows < 1 || k < 8 || n < 8 || rank < 8 || rank > 128 || adapters < 1) return 0;
-  return lora_bwd_space(rows, k, n, rank, adapters).total;
+extern "C" int64_t oga_lora_bwd_workspace_bytes(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters,
+                                                int64_t segments) {
+  if (rows < 1 || k < 8 || n < 8 || rank < 8 || rank > 128 || adapters < 1 || segments < 1) return 0;
+  return lora_bwd_space(rows, k, n, rank, adapters, segments).total;
 }
 
 extern "C" int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
@@ -599,11 +718,12 @@ extern "C" int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, cons
   if (!rows_ok(dy, dy_stride) || !rows_ok(x, x_stride) || !rows_ok(dx, dx_stride) || !rows_ok(a, k) ||
       !rows_ok(b, rank) || !rows_ok(low, 8) || !rows_ok(da, 8) || !rows_ok(db, 8))
     return fail("operand alignment");
-  const LoraBwdSpace w = lora_bwd_space(rows, k, n, rank, adapters);
+  const LoraBwdSpace w = lora_bwd_space(rows, k, n, rank, adapters, segments);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < w.total)
     return fail("workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)w.total);
   char* const ws = (char*)workspace;
-  float* const dlow = (float*)(ws + w.dlow);
+  float* const parts = (float*)ws;
+  float* const dlow = (float*)(ws + w.dlow);  // the parts themselves where there is one
   const hipStream_t s = (hipStream_t)stream;
 
   TransposeArgs t = {};
@@ -617,8 +737,9 @@ extern "C" int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, cons
   k_lora_transpose<<<dim3((unsigned)(adapters * (t.tiles[0] + t.tiles[1]))), dim3(256), 0, s>>>(t);
 
   const Segments g = {segment_starts, segment_adapters, (int)segments, (int)adapters, rows};
-  const ShrinkArgs sa = {g, dy, dy_stride, ws + w.bt, scale, dlow, n, (int)rank};
-  const ExpandArgs ea = {g, dlow, ws + w.at, nullptr, dx, 0, dx_stride, k, (int)rank, 0};
+  const ShrinkArgs sa = {g, dy, dy_stride, ws + w.bt, scale, parts, n, (int)rank};
+  const ExpandArgs ea = {g, parts, w.parts > 1 ? dlow : nullptr, ws + w.at, nullptr, dx, 0, dx_stride, k, (int)rank,
+                         w.parts};
   WgradArgs wa = {};
   wa.g = g, wa.rank = (int)rank, wa.splits = w.splits;
   wa.side[0] = {x, x_stride, dlow, k, (float*)(ws + w.pa), (int)((k + 511) / 512)};
@@ -631,12 +752,12 @@ extern "C" int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, cons
   j.blocks0 = (adapters * rank * k / 4 + 255) / 256;
   const dim3 jgrid((unsigned)(j.blocks0 + (adapters * rank * n / 4 + 255) / 256));
   if (x_dtype == OGA_DT_F16) {
-    shrink<OGA_DT_F16>(sa, s);
+    shrink<OGA_DT_F16>(sa, w.parts, s);
     expand<OGA_DT_F16>(ea, s);
     wgrad<OGA_DT_F16>(wa, s);
     k_lora_join<OGA_DT_F16><<<jgrid, dim3(256), 0, s>>>(j);
   } else {
-    shrink<OGA_DT_BF16>(sa, s);
+    shrink<OGA_DT_BF16>(sa, w.parts, s);
     expand<OGA_DT_BF16>(ea, s);
     wgrad<OGA_DT_BF16>(wa, s);
     k_lora_join<OGA_DT_BF16><<<jgrid, dim3(256), 0, s>>>(j);

@@ -151,6 +151,7 @@ PyMethodDef kMethods[] = {
     OGA_FN(oga_head_rmsnorm_rope),
     OGA_FN(oga_head_rmsnorm_rope_bwd_workspace_bytes),
     OGA_FN(oga_head_rmsnorm_rope_bwd),
+    OGA_FN(oga_lora_add_workspace_bytes),
     OGA_FN(oga_lora_add),
     OGA_FN(oga_lora_bwd_workspace_bytes),
     OGA_FN(oga_lora_bwd),

@@ -132,14 +132,16 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         out = torch.empty(y.shape, device=y.device, dtype=y.dtype)
     x2, xs = rows_layout(x)
     y2, ys = rows_layout(y)
-    low = torch.empty((rows, rank), device=x.device, dtype=torch.float32)
+    low = torch.empty((rows, rank), device=x.device, dtype=torch.float32) if save_low else None
     a, b = _packed(a), _packed(b)
     scale = None if scale is None else scale.contiguous()
     starts, ids = _i32(segment_starts, rows), _i32(segment_adapters, a.shape[0])
+    size = bytes_on(x, "oga_lora_add_workspace_bytes", rows, k, rank, ids.shape[0])
+    ws = torch.empty((size,), device=x.device, dtype=torch.uint8)
     _hip("lora_add")
     call_on(x, "oga_lora_add", _xdt(x), y2.data_ptr(), ys, x2.data_ptr(), xs, a.data_ptr(), b.data_ptr(),
             None if scale is None else scale.data_ptr(), starts.data_ptr(), ids.data_ptr(), ids.shape[0], a.shape[0],
-            low.data_ptr(), out.data_ptr(), n, rows, k, n, rank)
+            None if low is None else low.data_ptr(), out.data_ptr(), n, rows, k, n, rank, ws.data_ptr(), size)
     return (out, low) if save_low else out
 
 
@@ -175,7 +177,7 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, low: torch.Tensor, a: torch
     scale = None if scale is None else scale.contiguous()
     starts, ids = _i32(segment_starts, rows), _i32(segment_adapters, a.shape[0])
     da, db = torch.empty_like(a), torch.empty_like(b)
-    size = bytes_on(x, "oga_lora_bwd_workspace_bytes", rows, k, n, rank, a.shape[0])
+    size = bytes_on(x, "oga_lora_bwd_workspace_bytes", rows, k, n, rank, a.shape[0], ids.shape[0])
     ws = torch.empty((size,), device=x.device, dtype=torch.uint8)
     _hip("lora_backward")
     call_on(x, "oga_lora_bwd", _xdt(x), dy2.data_ptr(), dys, x2.data_ptr(), xs, low.data_ptr(), a.data_ptr(),

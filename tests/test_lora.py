@@ -158,18 +158,22 @@ def test_entry_points_refuse_what_the_kernels_do_not_take():
     """Nothing is launched: every call here fails its argument checks."""
     lib, p = _lib.load(), 4096
 
-    def add(dt=0, y=p, ys=64, x=p, starts=p, ids=p, segments=1, adapters=1, low=p, rows=4, k=64, n=64, rank=8):
+    def add(dt=0, y=p, ys=64, x=p, starts=p, ids=p, segments=1, adapters=1, low=p, rows=4, k=64, n=64, rank=8,
+            ws=p, size=1 << 40):
         return lib.oga_lora_add(dt, y, ys, x, 64, p, p, None, starts, ids, segments, adapters, low, p, 64, rows, k, n,
-                                rank, None)
+                                rank, ws, size, None)
 
     for kw in ({"dt": 1}, {"y": None}, {"y": 4104}, {"ys": 60}, {"x": None}, {"starts": None}, {"ids": None},
-               {"starts": 4098}, {"segments": 0}, {"adapters": 0}, {"adapters": 5000}, {"low": None}, {"rows": 0},
+               {"starts": 4098}, {"segments": 0}, {"adapters": 0}, {"adapters": 5000}, {"low": 4104}, {"rows": 0},
                {"k": 60}, {"n": 4}, {"k": 0}):
         assert add(**kw) == -1, kw
     for kw in ({"rank": 4}, {"rank": 12}, {"rank": 136}, {"rows": 1 << 31}, {"n": 1 << 23}):
         assert add(**kw) == -2, kw
-    need = lib.oga_lora_bwd_workspace_bytes(4, 64, 64, 8, 1)
-    assert need > 0 and lib.oga_lora_bwd_workspace_bytes(4, 64, 64, 136, 1) == 0
+    need = lib.oga_lora_add_workspace_bytes(4, 64, 8, 1)
+    assert need > 0 and lib.oga_lora_add_workspace_bytes(4, 64, 136, 1) == 0
+    assert add(ws=None) == -1 and add(ws=p + 16) == -1 and add(size=need - 1) == -1
+    need = lib.oga_lora_bwd_workspace_bytes(4, 64, 64, 8, 1, 1)
+    assert need > 0 and lib.oga_lora_bwd_workspace_bytes(4, 64, 64, 136, 1, 1) == 0
 
     def bwd(ws, size):
         return lib.oga_lora_bwd(0, p, 64, p, 64, p, p, p, None, p, p, 1, 1, p, 64, p, p, 4, 64, 64, 8, ws, size, None)
