@@ -9,10 +9,13 @@ from . import _lib
 from .ltx_ops import _stream
 
 
+_device = torch._C._cuda_getDevice
+
+
 def call_on(t: torch.Tensor, name: str, *args) -> None:
     """_lib.call(name, *args, stream) on t's device and its current stream."""
     index = t.get_device()
-    if torch._C._cuda_getDevice() == index:
+    if _device() == index:
         _lib.call(name, *args, _stream(t))
     else:
         with torch.cuda.device(index):
@@ -22,7 +25,7 @@ def call_on(t: torch.Tensor, name: str, *args) -> None:
 def bytes_on(t: torch.Tensor, name: str, *args) -> int:
     """A workspace query, which may go by t's device."""
     index = t.get_device()
-    if torch._C._cuda_getDevice() == index:
+    if _device() == index:
         return _lib.function(name)(*args)
     with torch.cuda.device(index):
         return _lib.function(name)(*args)
@@ -30,13 +33,15 @@ def bytes_on(t: torch.Tensor, name: str, *args) -> int:
 
 def heads_layout(t: torch.Tensor, most: int = 1 << 62) -> tuple[torch.Tensor, tuple[int, int, int]]:
     """t [B, N, H, D] as the kernels read it, and its (batch, token, head)
-    strides: unit stride along D, 16-byte aligned rows, a token stride below
-    `most`; a copy where t is laid out otherwise (an expanded gradient, a
+    strides: unit stride along D, 16-byte aligned rows, token and head strides
+    below `most`; a copy where t is laid out otherwise (an expanded gradient, a
     transposed view, an odd offset). An axis of one element has stride 0."""
-    b, n, h, d = t.shape
     sb, sn, sh, sd = t.stride()
+    if sd == 1 and not (sb | sn | sh) & 7 and 0 <= sn < most and 0 <= sh < most and not t.data_ptr() & 15:
+        return t, (sb, sn, sh)
+    b, n, h, d = t.shape
     sb, sn, sh = sb if b > 1 else 0, sn if n > 1 else 0, sh if h > 1 else 0
-    if (sd != 1 and d > 1) or (sb | sn | sh) & 7 or t.data_ptr() & 15 or not 0 <= sn < most:
+    if (sd != 1 and d > 1) or (sb | sn | sh) & 7 or t.data_ptr() & 15 or not 0 <= sn < most or not 0 <= sh < most:
         t = t.clone(memory_format=torch.contiguous_format)
         sb, sn, sh = n * h * d, h * d, d
     return t, (sb, sn, sh)
@@ -45,9 +50,21 @@ def heads_layout(t: torch.Tensor, most: int = 1 << 62) -> tuple[torch.Tensor, tu
 def rows_layout(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """t (..., C) as rows of C, and the row stride: unit stride along C,
     16-byte aligned rows; a copy where t is laid out otherwise."""
-    r = t.reshape(-1, t.shape[-1])
-    stride = r.stride(0) if r.shape[0] > 1 else 0
-    if r.stride(1) != 1 or stride & 7 or r.data_ptr() & 15:
-        r = r.clone(memory_format=torch.contiguous_format)
-        stride = r.stride(0)
-    return r, stride
+    if t.ndim != 2:
+        t = t.reshape(-1, t.shape[-1])
+    stride, unit = t.stride()
+    if unit != 1 or stride & 7 or t.data_ptr() & 15:
+        if t.shape[0] == 1 and (unit == 1 or t.shape[1] == 1) and not t.data_ptr() & 15:
+            return t, 0
+        t = t.clone(memory_format=torch.contiguous_format)
+        stride = t.stride(0)
+    return t, stride
+
+
+def vector32(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """t as a contiguous vector of dtype on a 32-byte boundary."""
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    if not t.is_contiguous() or t.data_ptr() & 31:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t

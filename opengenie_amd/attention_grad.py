@@ -31,34 +31,40 @@ __all__ = ["flash_attn_lse", "flash_attn_backward", "attention_with_grad"]
 _MOST = 1 << 24  # token strides the kernels take
 
 
-def _check(q, k, v, k_lens) -> None:
-    if q.ndim != 4 or k.ndim != 4 or k.shape != v.shape:
-        raise ValueError(f"attention shapes q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    if q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3] or not k.shape[2] or q.shape[2] % k.shape[2]:
-        raise ValueError(f"attention shapes q {tuple(q.shape)}, k {tuple(k.shape)}")
-    if q.dtype != k.dtype or q.dtype != v.dtype or not q.is_floating_point():
-        raise ValueError(f"attention dtypes q {q.dtype}, k {k.dtype}, v {v.dtype}")
-    if q.device != k.device or q.device != v.device:
+def _check(q, k, v, k_lens):
+    """The shapes (b, nq, h, d, nk, hk) of a call whose tensors fit each other."""
+    qs, ks, dtype, device = q.shape, k.shape, q.dtype, q.device
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape:
+        raise ValueError(f"attention shapes q {tuple(qs)}, k {tuple(ks)}, v {tuple(v.shape)}")
+    b, nq, h, d = qs
+    kb, nk, hk, kd = ks
+    if b != kb or d != kd or not hk or h % hk:
+        raise ValueError(f"attention shapes q {tuple(qs)}, k {tuple(ks)}")
+    if dtype != k.dtype or dtype != v.dtype or not dtype.is_floating_point:
+        raise ValueError(f"attention dtypes q {dtype}, k {k.dtype}, v {v.dtype}")
+    if device != k.device or device != v.device:
         raise ValueError("attention inputs on different devices")
     if k_lens is not None:
-        if k_lens.shape != (q.shape[0],) or k_lens.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"k_lens {k_lens.dtype} {tuple(k_lens.shape)} for a batch of {q.shape[0]}")
-        if k_lens.device != q.device:
+        if k_lens.shape != (b,) or (k_lens.dtype != torch.int32 and k_lens.dtype != torch.int64):
+            raise ValueError(f"k_lens {k_lens.dtype} {tuple(k_lens.shape)} for a batch of {b}")
+        if k_lens.device != device:
             raise ValueError("k_lens on another device")
+    return b, nq, h, d, nk, hk
 
 
 def _check_grad(dout, q, out, lse) -> None:
-    if dout.shape != q.shape or out.shape != q.shape or dout.dtype != q.dtype or out.dtype != q.dtype:
-        raise ValueError(f"dout {dout.dtype} {tuple(dout.shape)}, out {out.dtype} {tuple(out.shape)} for q {q.dtype} "
-                         f"{tuple(q.shape)}")
-    if lse.shape != (q.shape[0], q.shape[2], q.shape[1]):
-        raise ValueError(f"lse {tuple(lse.shape)} for q {tuple(q.shape)}")
-    if dout.device != q.device or out.device != q.device or lse.device != q.device:
+    shape, dtype, device = q.shape, q.dtype, q.device
+    if dout.shape != shape or out.shape != shape or dout.dtype != dtype or out.dtype != dtype:
+        raise ValueError(f"dout {dout.dtype} {tuple(dout.shape)}, out {out.dtype} {tuple(out.shape)} for q {dtype} "
+                         f"{tuple(shape)}")
+    if lse.shape != (shape[0], shape[2], shape[1]):
+        raise ValueError(f"lse {tuple(lse.shape)} for q {tuple(shape)}")
+    if dout.device != device or out.device != device or lse.device != device:
         raise ValueError("attention inputs on different devices")
 
 
-def _kernel_ok(q, k, scale: float) -> bool:
-    return q.is_cuda and q.dtype == torch.bfloat16 and q.shape[3] in (64, 128) and 0.0 < scale < 1e30
+def _kernel_ok(q, d: int, scale: float) -> bool:
+    return q.is_cuda and q.dtype == torch.bfloat16 and (d == 64 or d == 128) and 0.0 < scale < 1e30
 
 
 def _lens32(k_lens: torch.Tensor | None, nk: int) -> torch.Tensor | None:
@@ -66,7 +72,7 @@ def _lens32(k_lens: torch.Tensor | None, nk: int) -> torch.Tensor | None:
         return None
     if k_lens.dtype != torch.int32:
         k_lens = k_lens.clamp(0, nk).to(torch.int32)
-    return k_lens.contiguous()
+    return k_lens if k_lens.is_contiguous() else k_lens.contiguous()
 
 
 def _torch_inputs(q, k, v, causal, k_lens):
@@ -118,27 +124,27 @@ def flash_attn_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_sc
                    causal: bool = False, k_lens: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """out [B, Nq, H, D] and the float32 row log-sum-exp [B, H, Nq] of
     softmax(q k^T * scale) v, for `flash_attn_backward`."""
-    _check(q, k, v, k_lens)
-    b, nq, h, d = q.shape
-    nk, hk = k.shape[1], k.shape[2]
+    b, nq, h, d, nk, hk = _check(q, k, v, k_lens)
     scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
-    if q.numel() == 0 or nk == 0:
+    if not (b and nq and h and d and nk):
         dt = torch.float64 if q.dtype == torch.float64 else torch.float32
-        return torch.zeros_like(q, memory_format=torch.contiguous_format), torch.full((b, h, nq), -math.inf, device=q.device, dtype=dt)
-    if not _kernel_ok(q, k, scale):
+        return (torch.zeros_like(q, memory_format=torch.contiguous_format),
+                torch.full((b, h, nq), -math.inf, device=q.device, dtype=dt))
+    if not _kernel_ok(q, d, scale):
         _fallback("flash_attn_lse", q, k, v)
         return _torch_lse(q, k, v, scale, causal, k_lens)
     q, qs = heads_layout(q, _MOST)
     k, ks = heads_layout(k, _MOST)
     v, vs = heads_layout(v, _MOST)
     lens = _lens32(k_lens, nk)
-    out = torch.empty((b, nq, h, d), device=q.device, dtype=torch.bfloat16)
-    lse = torch.empty((b, h, nq), device=q.device, dtype=torch.float32)
-    size = bytes_on(q, "oga_attention_lse_workspace_bytes", b, nq, nk, h, hk, d, int(causal))
-    ws = torch.empty((size,), device=q.device, dtype=torch.uint8) if size else None
+    dev = q.device
+    out = torch.empty((b, nq, h, d), device=dev, dtype=torch.bfloat16)
+    lse = torch.empty((b, h, nq), device=dev, dtype=torch.float32)
+    size = bytes_on(q, "oga_attention_lse_workspace_bytes", b, nq, nk, h, hk, d, bool(causal))
+    ws = torch.empty((size,), device=dev, dtype=torch.uint8) if size else None
     _hip("flash_attn_lse")
     call_on(q, "oga_attention_lse", q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(),
-            (nq * h * d, h * d, d), lse.data_ptr(), b, nq, nk, h, hk, d, scale, int(causal),
+            (nq * h * d, h * d, d), lse.data_ptr(), b, nq, nk, h, hk, d, scale, bool(causal),
             None if lens is None else lens.data_ptr(), None if ws is None else ws.data_ptr(), size)
     return out, lse
 
@@ -148,14 +154,12 @@ def flash_attn_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v:
                         k_lens: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """dq, dk, dv of the call of `flash_attn_lse` that gave `out` and `lse`
     with these arguments. Deterministic: no sum goes through atomics."""
-    _check(q, k, v, k_lens)
+    b, nq, h, d, nk, hk = _check(q, k, v, k_lens)
     _check_grad(dout, q, out, lse)
-    b, nq, h, d = q.shape
-    nk, hk = k.shape[1], k.shape[2]
     scale = d ** -0.5 if softmax_scale is None else float(softmax_scale)
-    if q.numel() == 0 or nk == 0:
+    if not (b and nq and h and d and nk):
         return tuple(torch.zeros_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
-    if not _kernel_ok(q, k, scale) or lse.dtype != torch.float32:
+    if not _kernel_ok(q, d, scale) or lse.dtype != torch.float32:
         _fallback("flash_attn_backward", q, k, v)
         return _torch_backward(dout, q, k, v, out, lse, scale, causal, k_lens)
     q, qs = heads_layout(q, _MOST)
@@ -163,18 +167,20 @@ def flash_attn_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v:
     v, vs = heads_layout(v, _MOST)
     out, os = heads_layout(out, _MOST)
     dout, ds = heads_layout(dout, _MOST)
-    lse = lse.contiguous()
+    if not lse.is_contiguous():
+        lse = lse.contiguous()
     lens = _lens32(k_lens, nk)
-    dq = torch.empty((b, nq, h, d), device=q.device, dtype=torch.bfloat16)
-    dk = torch.empty((b, nk, hk, d), device=q.device, dtype=torch.bfloat16)
+    dev = q.device
+    dq = torch.empty((b, nq, h, d), device=dev, dtype=torch.bfloat16)
+    dk = torch.empty((b, nk, hk, d), device=dev, dtype=torch.bfloat16)
     dv = torch.empty_like(dk)
     dqs, dks = (nq * h * d, h * d, d), (nk * hk * d, hk * d, d)
-    size = bytes_on(q, "oga_attention_bwd_workspace_bytes", b, nq, nk, h, hk, d, int(causal))
-    ws = torch.empty((size,), device=q.device, dtype=torch.uint8)
+    size = bytes_on(q, "oga_attention_bwd_workspace_bytes", b, nq, nk, h, hk, d, bool(causal))
+    ws = torch.empty((size,), device=dev, dtype=torch.uint8)
     _hip("flash_attn_backward")
     call_on(q, "oga_attention_bwd", dout.data_ptr(), ds, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
             out.data_ptr(), os, lse.data_ptr(), dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(), dks, b, nq, nk,
-            h, hk, d, scale, int(causal), None if lens is None else lens.data_ptr(), ws.data_ptr(), size)
+            h, hk, d, scale, bool(causal), None if lens is None else lens.data_ptr(), ws.data_ptr(), size)
     return dq, dk, dv
 
 

@@ -83,28 +83,29 @@ struct Pair {
   int adapter;            // -1: none
 };
 
-// Pair number p for tiles of BM rows. Lanes test 64 segments at a time.
+// Pair number p for tiles of BM rows. Lanes test 64 segments at a time, each
+// with its bounds and adapter loaded side by side (one memory latency).
 template <int BM>
 OGA_DEVICE Pair seg_pair(const Segments& g, int64_t p, int lane) {
   const int all = g.count + 2;
-  int seg = 0;
-  int64_t b0 = 0;
+  int seg = 0, b0 = 0, b1 = 0, id = -1;
   for (int s0 = 0; s0 < all; s0 += 64) {
     const int s = s0 + lane;
-    const int64_t b = s < all ? seg_bound(g, s) : 0;
-    const unsigned long long m = __ballot(s < all && b / BM + s <= p);
+    const int lo = (int)seg_bound(g, s), hi = (int)seg_bound(g, s + 1);  // (rows stay below 2^31)
+    const int own = s >= 1 && s <= g.count ? g.ids[s - 1] : -1;
+    const unsigned long long m = __ballot(s < all && lo / BM + s <= p);
     if (!m) break;
     const int top = 63 - __builtin_clzll(m);
     seg = s0 + top;
-    b0 = (int64_t)__builtin_amdgcn_readlane((int)b, top);  // rows stay below 2^31
+    b0 = __builtin_amdgcn_readlane(lo, top);
+    b1 = __builtin_amdgcn_readlane(hi, top);
+    id = __builtin_amdgcn_readlane(own, top);
     if (top < 63) break;
   }
-  const int64_t b1 = seg_bound(g, seg + 1);
   Pair r;
   r.tile0 = (p - seg) * BM;  // floor(b0 / BM) + j tiles down
-  r.lo = max(b0, r.tile0);
-  r.hi = min(b1, r.tile0 + BM);
-  const int id = seg >= 1 && seg <= g.count ? g.ids[seg - 1] : -1;
+  r.lo = max((int64_t)b0, r.tile0);
+  r.hi = min((int64_t)b1, r.tile0 + BM);
   r.adapter = id >= 0 && id < g.adapters ? id : -1;
   return r;
 }
@@ -172,16 +173,36 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void k_lora_shrink(ShrinkArgs a)
 #pragma unroll
         for (int t = 0; t < TB; ++t) acc[t][r] = mfma16<XDT>(f.w[h][r], f.x[h][t], acc[t][r]);
   };
+  // (no load behind a branch inside the loop: the wait before its products
+  // would then be for every load)
   const int end = min(c1, whole);
   Chunk f0, f1;
-  int ch = c0 + wv;
-  if (ch < end) load(f0, ch);
-  for (; ch < end; ch += 2 * kShrinkWaves) {
-    const bool two = ch + kShrinkWaves < end;
-    if (two) load(f1, ch + kShrinkWaves);
-    mul(f0);
-    if (ch + 2 * kShrinkWaves < end) load(f0, ch + 2 * kShrinkWaves);
-    if (two) mul(f1);
+  // This wave's n chunks, c0 + wv + 4 i, beginning with i = first: all tiles
+  // would otherwise read the same columns of their rows at one time, which are
+  // powers of two apart and so in the same few memory channels.
+  const int n = end > c0 + wv ? (end - c0 - wv + kShrinkWaves - 1) / kShrinkWaves : 0;
+  int ch = n ? c0 + wv + kShrinkWaves * (int)(blockIdx.x % (uint32_t)n) : 0;
+  auto next = [&] {
+    const int now = ch;
+    ch = ch + kShrinkWaves < end ? ch + kShrinkWaves : c0 + wv;
+    return now;
+  };
+  if (n) {
+    load(f0, next());
+    int i = 2;
+    for (; i < n; i += 2) {
+      load(f1, next());
+      mul(f0);
+      load(f0, next());
+      mul(f1);
+    }
+    if (i == n) {
+      load(f1, next());
+      mul(f0);
+      mul(f1);
+    } else {
+      mul(f0);
+    }
   }
   if (c1 > whole && wv == (whole - c0) % kShrinkWaves) {  // the last 8 .. 56 of the axis
     const uint4 none = make_uint4(0, 0, 0, 0);
@@ -189,9 +210,15 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void k_lora_shrink(ShrinkArgs a)
     for (int h = 0; h < 2; ++h) {
       const bool in = 64 * whole + 32 * h + kg < a.k;
 #pragma unroll
-      for (int t = 0; t < TB; ++t) f0.x[h][t] = in ? *(const uint4*)(xr[t] + 64 * whole + 32 * h) : none;
+      for (int t = 0; t < TB; ++t) {
+        f0.x[h][t] = none;
+        if (in) f0.x[h][t] = *(const uint4*)(xr[t] + 64 * whole + 32 * h);
+      }
 #pragma unroll
-      for (int r = 0; r < RB; ++r) f0.w[h][r] = in ? *(const uint4*)(wr[r] + 64 * whole + 32 * h) : none;
+      for (int r = 0; r < RB; ++r) {
+        f0.w[h][r] = none;
+        if (in) f0.w[h][r] = *(const uint4*)(wr[r] + 64 * whole + 32 * h);
+      }
     }
     mul(f0);
   }
@@ -223,45 +250,62 @@ struct ExpandArgs {
   int64_t ys, os;    // row strides
   int64_t n;
   int rank, parts;
+  uint32_t col_blocks;
 };
 
-constexpr int kExpandWaves = 4;
-
-#ifndef OGA_EXP_PF
-#define OGA_EXP_PF 0
-#endif
-#ifndef OGA_EXP_G
-#define OGA_EXP_G 4
-#endif
-// 16 TB rows x 32 G columns per wave. The features of the two MFMA row blocks
-// of a 32-column group interleave by fours (block b's row 4g + i is column
-// 8g + 4b + i), so a lane ends with 8 consecutive columns of its row. The two
-// halves of the tile's low, which all waves use, go through LDS as fragments.
-template <int XDT, int KS, int TB, int G>
-__global__ __launch_bounds__(64 * kExpandWaves) void k_lora_expand(ExpandArgs a) {
+// 16 TB rows x 128 columns per wave: operand A is low (16 rows, its two halves
+// as fragments in LDS, shared by the waves), operand B of product j the eight
+// columns' j-th, 8 (l % 16) + j for lane l, so that a lane ends with 8
+// consecutive columns of 4 rows and y moves in pieces of 256 bytes a row (16
+// rows x 64 bytes at a time, as the other orientation has it, moved 2.9 TB/s).
+template <int XDT, int KS, int TB, int W>
+__global__ __launch_bounds__(64 * W) void k_lora_expand(ExpandArgs a) {
   __shared__ uint4 lows[TB][KS][2][64];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const Pair p = seg_pair<16 * TB>(a.g, blockIdx.x, lane);
+  // column blocks in turn: the tile's low is read while it is in a cache
+  const uint32_t tile = blockIdx.x / a.col_blocks, col_block = blockIdx.x % a.col_blocks;
+  const Pair p = seg_pair<16 * TB>(a.g, tile, lane);
   if (p.hi <= p.lo) return;
-  const int c = lane & 15, kg = 8 * (lane >> 4);
-  const int64_t f_begin = ((int64_t)blockIdx.y * kExpandWaves + wv) * 32 * G;
-  const int64_t f_end = min(f_begin + 32 * G, a.n);
+  const int c = lane & 15, g4 = lane >> 4, kg = 8 * g4;
+  const int64_t f0 = ((int64_t)col_block * W + wv) * 128, f = f0 + 8 * c;  // this lane's 8 columns
+  const uint16_t* const y = (const uint16_t*)a.y;
+  uint16_t* const out = (uint16_t*)a.out;
+  const uint4 none = make_uint4(0, 0, 0, 0);
   if (p.adapter < 0) {  // rows without an adapter keep y (dx: zero)
-    if (a.y == a.out) return;
-    for (int64_t f = f_begin + kg; f < f_end; f += 32)
-#pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        const int64_t row = p.tile0 + 16 * t + c;
-        if (row < p.lo || row >= p.hi) continue;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (a.y) v = *(const uint4*)((const uint16_t*)a.y + row * a.ys + f);
-        *(uint4*)((uint16_t*)a.out + row * a.os + f) = v;
+    if (a.y == a.out || f >= a.n) return;
+    for (int64_t r = p.tile0 + g4; r < p.hi; r += 4)
+      if (r >= p.lo) {
+        uint4 v = none;
+        if (y) v = *(const uint4*)(y + r * a.ys + f);
+        *(uint4*)(out + r * a.os + f) = v;
       }
     return;
   }
+  // All of the wave's loads go out at once: y (rows 16 t + 4 g4 .. + 3), the
+  // weights' eight columns, and its share of low. (With y read 16 rows at a
+  // time, a workgroup's chain of loads took twice as long as the bytes need.)
+  uint4 yv[TB][4];
+  if (y) {
+#pragma unroll
+    for (int t = 0; t < TB; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t r = min(max(p.tile0 + 16 * t + 4 * g4 + i, p.lo), p.hi - 1);
+        yv[t][i] = *(const uint4*)(y + r * a.ys + min(f, a.n - 8));
+      }
+  }
+  uint4 w[8][KS];
+  {
+    const uint16_t* wa = (const uint16_t*)a.w + (int64_t)p.adapter * a.n * a.rank;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        w[j][s] = *(const uint4*)(wa + min(f + j, a.n - 1) * a.rank + min(32 * s + kg, a.rank - 8));
+  }
   // wave w takes fragments w, w + 4, ... of the tile's TB x KS
-  for (int u = wv; u < TB * KS; u += kExpandWaves) {
+  for (int u = wv; u < TB * KS; u += W) {
     const int t = u / KS, s = u % KS;
     const int64_t row = p.tile0 + 16 * t + c, rc = min(max(row, p.lo), p.hi - 1);
     float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -280,7 +324,7 @@ __global__ __launch_bounds__(64 * kExpandWaves) void k_lora_expand(ExpandArgs a)
         for (int e = 0; e < 4; ++e) add(x[e], y[e]);
       }
       for (; q < a.parts; ++q) add(*(const float4*)(l + q * step), *(const float4*)(l + q * step + 4));
-      if (a.low_sum && row == rc && blockIdx.y == 0) {
+      if (a.low_sum && row == rc && col_block == 0) {
         float* o = a.low_sum + row * a.rank + 32 * s + kg;
         *(float4*)o = make_float4(f[0], f[1], f[2], f[3]);
         *(float4*)(o + 4) = make_float4(f[4], f[5], f[6], f[7]);
@@ -292,64 +336,43 @@ __global__ __launch_bounds__(64 * kExpandWaves) void k_lora_expand(ExpandArgs a)
     lows[t][s][1][lane] = lo;
   }
   __syncthreads();
-  struct Group {
-    uint4 y[TB], w[2][KS];
-  };
-  const uint4 none = make_uint4(0, 0, 0, 0);
-  const uint16_t* w = (const uint16_t*)a.w + (int64_t)p.adapter * a.n * a.rank;
-  auto load = [&](Group& g, int64_t f0) {
-    if (a.y) {
+  if (f0 >= a.n) return;  // (no barrier follows)
+  if (a.rank < 32 * KS) {  // what is read past the rank counts as 0, whatever it holds
 #pragma unroll
-      for (int t = 0; t < TB; ++t)
-        g.y[t] = *(const uint4*)((const uint16_t*)a.y + min(max(p.tile0 + 16 * t + c, p.lo), p.hi - 1) * a.ys +
-                                 min(f0 + kg, a.n - 8));
-    }
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int64_t feat = min(f0 + 8 * (c >> 2) + 4 * b + (c & 3), a.n - 1);
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int s = 0; s < KS; ++s)
-        g.w[b][s] = 32 * s + kg < a.rank ? *(const uint4*)(w + feat * a.rank + 32 * s + kg) : none;
-    }
-  };
-  Group cur, nxt;
-  if (OGA_EXP_PF && f_begin < f_end) load(cur, f_begin);
-#pragma unroll 1
-  for (int64_t f0 = f_begin; f0 < f_end; f0 += 32) {
-    const int64_t f = f0 + kg;  // this lane's 8 columns
-    if (!OGA_EXP_PF)
-      load(cur, f0);
-    else if (f0 + 32 < f_end)
-      load(nxt, f0 + 32);
-    f32x4 acc[2][TB];
+        if (32 * s + kg >= a.rank) w[j][s] = none;
+  }
 #pragma unroll
-    for (int t = 0; t < TB; ++t) {
+  for (int t = 0; t < TB; ++t) {
+    const int64_t r0 = p.tile0 + 16 * t;
+    if (r0 >= p.hi || r0 + 16 <= p.lo) continue;
+    f32x4 acc[8];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) acc[b][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < 8; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int h = 1; h >= 0; --h) {
-          const uint4 l = lows[t][s][h][lane];
+      for (int h = 1; h >= 0; --h) {
+        const uint4 l = lows[t][s][h][lane];
 #pragma unroll
-          for (int b = 0; b < 2; ++b) acc[b][t] = mfma16<XDT>(cur.w[b][s], l, acc[b][t]);
-        }
-    }
+        for (int j = 0; j < 8; ++j) acc[j] = mfma16<XDT>(l, w[j][s], acc[j]);
+      }
 #pragma unroll
-    for (int t = 0; t < TB; ++t) {
-      const int64_t row = p.tile0 + 16 * t + c;
-      float v[8];
-      if (a.y) {
-        unpack8x<XDT>(cur.y[t], v);
+    for (int i = 0; i < 4; ++i) {
+      float o[8];
+      if (y) {
+        unpack8x<XDT>(yv[t][i], o);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += acc[i >> 2][t][i & 3];
+        for (int j = 0; j < 8; ++j) o[j] += acc[j][i];
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = acc[i >> 2][t][i & 3];
+        for (int j = 0; j < 8; ++j) o[j] = acc[j][i];
       }
-      if (row >= p.lo && row < p.hi && f < a.n) *(uint4*)((uint16_t*)a.out + row * a.os + f) = pack8x<XDT>(v);
+      const int64_t r = r0 + 4 * g4 + i;
+      if (r >= p.lo && r < p.hi && f < a.n) st_nt16(out + r * a.os + f, pack8x<XDT>(o));
     }
-    if (OGA_EXP_PF) cur = nxt;
   }
 }
 
@@ -430,12 +453,9 @@ __global__ __launch_bounds__(256) void k_lora_wgrad(WgradArgs a) {
   auto tile = [&](int64_t lo, int64_t hi) {
     const int steps = (int)((min(hi - lo, (int64_t)kWgradRows) + 31) / 32);
     auto rows8 = [&](Rows8& x, int64_t first) {
-      const int64_t row = first + g8;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x.v[j] = make_uint4(0, 0, 0, 0);  // rows of others may hold anything
-        if (row + j < hi) x.v[j] = *(const uint4*)((const uint16_t*)sd.x + (row + j) * sd.xs + colc);
-      }
+      for (int j = 0; j < 8; ++j)
+        x.v[j] = *(const uint4*)((const uint16_t*)sd.x + min(first + g8 + j, hi - 1) * sd.xs + colc);
     };
     Rows8 cur, nxt;
     rows8(cur, lo);  // in flight while the tile's u goes to LDS
@@ -455,7 +475,12 @@ __global__ __launch_bounds__(256) void k_lora_wgrad(WgradArgs a) {
     }
     __syncthreads();
     for (int st = 0; st < steps; ++st) {
-      if (st + 1 < steps) rows8(nxt, lo + 32 * (st + 1));
+      rows8(nxt, lo + 32 * (st + 1));  // (past the end: the last row again)
+      if (lo + 32 * st + 32 > hi) {    // rows of others may hold anything
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (lo + 32 * st + g8 + j >= hi) cur.v[j] = make_uint4(0, 0, 0, 0);
+      }
       uint4 fh[RB], fl[RB];
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
@@ -549,11 +574,19 @@ static int row_blocks(const Segments& g, int most) {
   return mean >= 48 ? most : mean >= 16 ? min(most, 2) : 1;
 }
 
-// Parts of the long axis: enough workgroups for four a CU, each wave with two
-// chunks or more.
+// Parts of the long axis: with three workgroups a CU at a time, the number
+// whose rounds times a part's length is least (each wave with two chunks or
+// more).
 static int shrink_parts(int64_t rows, int64_t segments, int64_t k) {
-  const int64_t pairs = seg_pairs(rows, segments, rows / segments >= 16 ? 32 : 16);
-  return (int)max((int64_t)1, min(min(4 * (int64_t)cu_count() / pairs, (k + 63) / 64 / (2 * kShrinkWaves)), (int64_t)8));
+  const int64_t pairs = seg_pairs(rows, segments, rows / segments >= 16 ? 32 : 16), slots = 3 * (int64_t)cu_count();
+  const int64_t most = min((k + 63) / 64 / (2 * kShrinkWaves), (int64_t)8);
+  int best = 1;
+  double least = 1e30;
+  for (int p = 1; p <= most; ++p) {
+    const double cost = (double)((pairs * p + slots - 1) / slots) / p + 0.01 * p;
+    if (cost < least) least = cost, best = p;
+  }
+  return best;
 }
 
 template <int XDT, int RB>
@@ -577,22 +610,22 @@ static void shrink(const ShrinkArgs& a, int parts, hipStream_t s) {
     shrink_launch<XDT, 8>(a, parts, s);
 }
 
-template <int XDT, int KS, int TB, int G>
-static void expand_launch(const ExpandArgs& a, hipStream_t s) {
-  constexpr int cols = 32 * G * kExpandWaves;
-  const dim3 grid((unsigned)seg_pairs(a.g.rows, a.g.count, 16 * TB), (unsigned)((a.n + cols - 1) / cols));
-  k_lora_expand<XDT, KS, TB, G><<<grid, dim3(64 * kExpandWaves), 0, s>>>(a);
+template <int XDT, int KS, int TB, int W>
+static void expand_launch(ExpandArgs a, hipStream_t s) {
+  a.col_blocks = (uint32_t)((a.n + 128 * W - 1) / (128 * W));
+  const dim3 grid((unsigned)(seg_pairs(a.g.rows, a.g.count, 16 * TB) * a.col_blocks));
+  k_lora_expand<XDT, KS, TB, W><<<grid, dim3(64 * W), 0, s>>>(a);
 }
 template <int XDT, int KS>
 static void expand_rows(const ExpandArgs& a, hipStream_t s) {
   constexpr int most = KS >= 4 ? 2 : 4;
   const int tb = row_blocks(a.g, most);
   if (tb == 4)
-    expand_launch<XDT, KS, most, OGA_EXP_G>(a, s);
+    expand_launch<XDT, KS, most, 8>(a, s);
   else if (tb == 2)
-    expand_launch<XDT, KS, 2, OGA_EXP_G>(a, s);
+    expand_launch<XDT, KS, 2, 8>(a, s);
   else
-    expand_launch<XDT, KS, 1, 1>(a, s);
+    expand_launch<XDT, KS, 1, 4>(a, s);
 }
 template <int XDT>
 static void expand(const ExpandArgs& a, hipStream_t s) {
@@ -691,7 +724,7 @@ extern "C" int oga_lora_add(int x_dtype, const void* y, int64_t y_stride, const 
   const Segments g = {segment_starts, segment_adapters, (int)segments, (int)adapters, rows};
   const int parts = shrink_parts(rows, segments, k);
   const ShrinkArgs sa = {g, x, x_stride, a, scale, (float*)workspace, k, (int)rank};
-  const ExpandArgs ea = {g, (const float*)workspace, low, b, y, out, y_stride, out_stride, n, (int)rank, parts};
+  const ExpandArgs ea = {g, (const float*)workspace, low, b, y, out, y_stride, out_stride, n, (int)rank, parts, 0};
   const hipStream_t s = (hipStream_t)stream;
   if (x_dtype == OGA_DT_F16) {
     shrink<OGA_DT_F16>(sa, parts, s);
@@ -739,7 +772,7 @@ extern "C" int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, cons
   const Segments g = {segment_starts, segment_adapters, (int)segments, (int)adapters, rows};
   const ShrinkArgs sa = {g, dy, dy_stride, ws + w.bt, scale, parts, n, (int)rank};
   const ExpandArgs ea = {g, parts, w.parts > 1 ? dlow : nullptr, ws + w.at, nullptr, dx, 0, dx_stride, k, (int)rank,
-                         w.parts};
+                         w.parts, 0};
   WgradArgs wa = {};
   wa.g = g, wa.rank = (int)rank, wa.splits = w.splits;
   wa.side[0] = {x, x_stride, dlow, k, (float*)(ws + w.pa), (int)((k + 511) / 512)};

@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import torch
 
-from ._launch import bytes_on, call_on, heads_layout
+from ._launch import bytes_on, call_on, heads_layout, vector32
 from .ltx_ops import _any_dt, _fallback, _hip, _xdt
 
 __all__ = ["qk_head_rmsnorm_rope", "qk_head_rmsnorm_rope_backward", "qk_head_rmsnorm_rope_with_grad", "apply_rope"]
@@ -30,66 +30,63 @@ _PARAM = (torch.bfloat16, torch.float32)
 
 
 def _check(x, k, cos, sin, layout, positions) -> None:
-    if layout not in ("half", "interleaved"):
+    if layout != "half" and layout != "interleaved":
         raise ValueError(f"unknown rotary layout: {layout}")
-    if x.ndim != 4 or not x.is_floating_point():
-        raise ValueError(f"heads {x.dtype} {tuple(x.shape)}")
-    if k is not None and (k.ndim != 4 or k.shape[:2] != x.shape[:2] or k.shape[3] != x.shape[3] or k.dtype != x.dtype
-                          or k.device != x.device):
-        raise ValueError(f"k {k.dtype} {tuple(k.shape)} beside q {x.dtype} {tuple(x.shape)}")
-    if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or not 0 < 2 * cos.shape[1] <= x.shape[3]:
-        raise ValueError(f"cos {tuple(cos.shape)}, sin {tuple(sin.shape)} for heads of {x.shape[3]}")
-    if cos.device != x.device or sin.device != x.device:
+    shape, dtype, device, table = x.shape, x.dtype, x.device, cos.shape
+    if len(shape) != 4 or not dtype.is_floating_point:
+        raise ValueError(f"heads {dtype} {tuple(shape)}")
+    if k is not None:
+        other = k.shape
+        if (len(other) != 4 or other[0] != shape[0] or other[1] != shape[1] or other[3] != shape[3]
+                or k.dtype != dtype or k.device != device):
+            raise ValueError(f"k {k.dtype} {tuple(other)} beside q {dtype} {tuple(shape)}")
+    if len(table) != 2 or table != sin.shape or cos.dtype != sin.dtype or not 0 < 2 * table[1] <= shape[3]:
+        raise ValueError(f"cos {tuple(table)}, sin {tuple(sin.shape)} for heads of {shape[3]}")
+    if cos.device != device or sin.device != device:
         raise ValueError("cos/sin on another device")
     if positions is None:
-        if cos.shape[0] < x.shape[1]:
-            raise ValueError(f"cos/sin of {cos.shape[0]} positions for {x.shape[1]} tokens")
+        if table[0] < shape[1]:
+            raise ValueError(f"cos/sin of {table[0]} positions for {shape[1]} tokens")
     else:
-        if positions.shape != x.shape[:2] or positions.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"positions {positions.dtype} {tuple(positions.shape)} for {tuple(x.shape[:2])} tokens")
-        if positions.device != x.device:
+        if positions.shape != shape[:2] or (positions.dtype != torch.int32 and positions.dtype != torch.int64):
+            raise ValueError(f"positions {positions.dtype} {tuple(positions.shape)} for {tuple(shape[:2])} tokens")
+        if positions.device != device:
             raise ValueError("positions on another device")
-        if cos.shape[0] < 1:
+        if table[0] < 1:
             raise ValueError("cos/sin without positions")
 
 
-def _check_weights(q, q_weight, k_weight) -> None:
-    for w in (q_weight, k_weight):
-        if w is not None and (w.shape != q.shape[3:] or w.device != q.device or not w.is_floating_point()):
-            raise ValueError(f"weight {w.dtype} {tuple(w.shape)} for heads of {q.shape[3]}")
+def _check_weight(q, w) -> None:
+    if w is not None and (w.shape != q.shape[3:] or w.device != q.device or not w.dtype.is_floating_point):
+        raise ValueError(f"weight {w.dtype} {tuple(w.shape)} for heads of {q.shape[3]}")
 
 
-def _kernel_ok(x, cos, *weights) -> bool:
-    return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and x.shape[3] in (64, 128, 256)
-            and cos.shape[1] % 8 == 0 and cos.dtype in _PARAM
-            and all(w is None or w.dtype in _PARAM for w in weights))
-
-
-def _table(t: torch.Tensor) -> torch.Tensor:
-    """A table with rows the kernel reads 4 entries at a time."""
-    if t.stride(1) != 1 or t.stride(0) % 4 or t.stride(0) < 0 or t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+def _kernel_ok(x, cos, q_weight=None, k_weight=None) -> bool:
+    return (x.is_cuda and (x.dtype == torch.bfloat16 or x.dtype == torch.float16) and x.shape[3] in (64, 128, 256)
+            and cos.shape[1] % 8 == 0 and cos.dtype in _PARAM and (q_weight is None or q_weight.dtype in _PARAM)
+            and (k_weight is None or k_weight.dtype in _PARAM))
 
 
 def _tables(cos, sin):
-    cos, sin = _table(cos), _table(sin)
-    if cos.stride(0) != sin.stride(0):
-        cos, sin = cos.contiguous(), sin.contiguous()
-    return cos, sin
+    """Tables with rows the kernel reads 4 entries at a time, and their row
+    stride."""
+    (row, unit), other = cos.stride(), sin.stride()
+    if unit != 1 or row & 3 or row < 0 or other != (row, 1) or cos.data_ptr() & 15 or sin.data_ptr() & 15:
+        cos, sin = (t.clone(memory_format=torch.contiguous_format) for t in (cos, sin))
+        row = cos.shape[1]
+    return cos, sin, row
 
 
-def _vector(w: torch.Tensor | None, dtype) -> torch.Tensor | None:
-    if w is None:
-        return None
-    w = w.to(dtype).contiguous()
-    return w if w.data_ptr() % 32 == 0 else w.clone()
-
-
-def _weight_dtype(q_weight, k_weight):
-    """One dtype for both weights: theirs, or float32 where they differ."""
-    dts = {w.dtype for w in (q_weight, k_weight) if w is not None}
-    return dts.pop() if len(dts) == 1 else torch.float32
+def _weights(q_weight, k_weight):
+    """Both weights as the kernels read them in one dtype: theirs, or float32
+    where they differ."""
+    if q_weight is None and k_weight is None:
+        return None, None, torch.float32
+    dtype = (k_weight if q_weight is None else q_weight).dtype
+    if q_weight is not None and k_weight is not None and k_weight.dtype != dtype:
+        dtype = torch.float32
+    return (None if q_weight is None else vector32(q_weight, dtype),
+            None if k_weight is None else vector32(k_weight, dtype), dtype)
 
 
 def _pos_args(positions):
@@ -142,22 +139,23 @@ def _torch_norm_turn_grad(dy, x, w, eps, cos, sin, layout):
 
 def _forward(q, k, q_weight, k_weight, eps, cos, sin, layout, positions, norm, inverse):
     b, n, h, d = q.shape
-    hk = 0 if k is None else k.shape[2]
     q, qs = heads_layout(q)
     q_out = torch.empty((b, n, h, d), device=q.device, dtype=q.dtype)
-    k_out, ks, kos = None, (0, 0, 0), (0, 0, 0)
+    hk, k_out, kp, kop, ks, kos = 0, None, None, None, (0, 0, 0), (0, 0, 0)
     if k is not None:
+        hk = k.shape[2]
         k, ks = heads_layout(k)
         k_out = torch.empty((b, n, hk, d), device=q.device, dtype=q.dtype)
         kos = (n * hk * d, hk * d, d)
-    wdt = _weight_dtype(q_weight, k_weight)
-    qw, kw = _vector(q_weight, wdt), _vector(k_weight, wdt)
-    cos, sin = _tables(cos, sin)
+        kp, kop = k.data_ptr(), k_out.data_ptr()
+    qw, kw, wdt = _weights(q_weight, k_weight)
+    cos, sin, row = _tables(cos, sin)
     pos, pos64, pos_strides = _pos_args(positions)
-    call_on(q, "oga_head_rmsnorm_rope", _xdt(q), q.data_ptr(), qs, _ptr(k), ks, _ptr(qw), _ptr(kw),
-            0 if wdt == torch.bfloat16 else 1, cos.data_ptr(), sin.data_ptr(), _any_dt(cos), cos.stride(0),
-            cos.shape[0], pos, pos64, pos_strides, q_out.data_ptr(), (n * h * d, h * d, d), _ptr(k_out), kos, b, n, h,
-            hk, d, 2 * cos.shape[1], int(layout == "interleaved"), int(inverse), int(norm), eps)
+    length, half = cos.shape
+    call_on(q, "oga_head_rmsnorm_rope", _xdt(q), q.data_ptr(), qs, kp, ks, _ptr(qw), _ptr(kw),
+            0 if wdt == torch.bfloat16 else 1, cos.data_ptr(), sin.data_ptr(), _any_dt(cos), row, length, pos, pos64,
+            pos_strides, q_out.data_ptr(), (n * h * d, h * d, d), kop, kos, b, n, h, hk, d, 2 * half,
+            layout == "interleaved", inverse, norm, eps)
     return q_out, k_out
 
 
@@ -166,8 +164,9 @@ def qk_head_rmsnorm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tenso
                          layout: str = "half", positions: torch.Tensor | None = None):
     """The normed and rotated q and k, in one pass over both."""
     _check(q, k, cos, sin, layout, positions)
-    _check_weights(q, q_weight, k_weight)
-    if q.numel() == 0 or k.numel() == 0 or not _kernel_ok(q, cos, q_weight, k_weight):
+    _check_weight(q, q_weight)
+    _check_weight(q, k_weight)
+    if not (q.numel() and k.numel() and _kernel_ok(q, cos, q_weight, k_weight)):
         if q.numel() and k.numel():
             _fallback("qk_head_rmsnorm_rope", q, k)
         c, s = _torch_tables(cos, sin, q.shape[1], positions, _wide(q))
@@ -184,11 +183,12 @@ def qk_head_rmsnorm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q:
     `qk_head_rmsnorm_rope` with these inputs, from its outputs' gradients. The
     weights' gradients are summed without atomics, in a fixed order."""
     _check(q, k, cos, sin, layout, positions)
-    _check_weights(q, q_weight, k_weight)
+    _check_weight(q, q_weight)
+    _check_weight(q, k_weight)
     for g, x in ((dq_out, q), (dk_out, k)):
         if g.shape != x.shape or g.dtype != x.dtype or g.device != x.device:
             raise ValueError(f"gradient {g.dtype} {tuple(g.shape)} of {x.dtype} {tuple(x.shape)}")
-    if q.numel() == 0 or k.numel() == 0 or not _kernel_ok(q, cos, q_weight, k_weight):
+    if not (q.numel() and k.numel() and _kernel_ok(q, cos, q_weight, k_weight)):
         if q.numel() and k.numel():
             _fallback("qk_head_rmsnorm_rope_backward", q, k)
         c, s = _torch_tables(cos, sin, q.shape[1], positions, _wide(q))
@@ -204,10 +204,9 @@ def qk_head_rmsnorm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q:
     dk_out, dkos = heads_layout(dk_out)
     dq = torch.empty((b, n, h, d), device=q.device, dtype=q.dtype)
     dk = torch.empty((b, n, hk, d), device=q.device, dtype=q.dtype)
-    wdt = _weight_dtype(q_weight, k_weight)
-    qw, kw = _vector(q_weight, wdt), _vector(k_weight, wdt)
+    qw, kw, wdt = _weights(q_weight, k_weight)
     dqw, dkw = (None if w is None else torch.empty((d,), device=q.device, dtype=wdt) for w in (qw, kw))
-    cos, sin = _tables(cos, sin)
+    cos, sin, row = _tables(cos, sin)
     pos, pos64, pos_strides = _pos_args(positions)
     ws, size = None, 0
     if qw is not None or kw is not None:
@@ -215,7 +214,7 @@ def qk_head_rmsnorm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q:
         ws = torch.empty((size,), device=q.device, dtype=torch.uint8)
     call_on(q, "oga_head_rmsnorm_rope_bwd", _xdt(q), dq_out.data_ptr(), dqos, dk_out.data_ptr(), dkos, q.data_ptr(),
             qs, k.data_ptr(), ks, _ptr(qw), _ptr(kw), 0 if wdt == torch.bfloat16 else 1, cos.data_ptr(),
-            sin.data_ptr(), _any_dt(cos), cos.stride(0), cos.shape[0], pos, pos64, pos_strides, dq.data_ptr(),
+            sin.data_ptr(), _any_dt(cos), row, cos.shape[0], pos, pos64, pos_strides, dq.data_ptr(),
             (n * h * d, h * d, d), dk.data_ptr(), (n * hk * d, hk * d, d), _ptr(dqw), _ptr(dkw), b, n, h, hk, d,
             2 * cos.shape[1], int(layout == "interleaved"), float(eps), _ptr(ws), size)
     if dqw is not None and dqw.dtype != q_weight.dtype:

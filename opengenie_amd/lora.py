@@ -30,6 +30,8 @@ import torch
 from ._launch import bytes_on, call_on, rows_layout
 from .ltx_ops import _fallback, _hip, _xdt, fp8_linear_forward
 
+_INDEX = (torch.int32, torch.int64)
+
 __all__ = ["LoraAdapters", "lora_add", "lora_backward", "lora_add_with_grad", "fp8_linear_lora_forward"]
 
 
@@ -52,37 +54,39 @@ class LoraAdapters:
                             torch.tensor([float(s) for _, _, s in adapters], device=adapters[0][0].device))
 
 
-def _check(x, n, a, b, scale, starts, ids) -> None:
-    if a.ndim != 3 or b.ndim != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or not a.numel():
-        raise ValueError(f"adapters a {tuple(a.shape)}, b {tuple(b.shape)}")
-    if a.shape[2] != x.shape[-1] or b.shape[1] != n:
-        raise ValueError(f"adapters a {tuple(a.shape)}, b {tuple(b.shape)} for {x.shape[-1]} -> {n}")
-    if a.dtype != x.dtype or b.dtype != x.dtype or not x.is_floating_point():
-        raise ValueError(f"dtypes x {x.dtype}, a {a.dtype}, b {b.dtype}")
-    if scale is not None and (scale.shape != a.shape[:1] or scale.dtype != torch.float32):
-        raise ValueError(f"scale {scale.dtype} {tuple(scale.shape)} of {a.shape[0]} adapters")
-    if (starts.ndim != 1 or ids.ndim != 1 or starts.shape[0] != ids.shape[0] + 1
-            or starts.dtype not in (torch.int32, torch.int64) or ids.dtype not in (torch.int32, torch.int64)):
-        raise ValueError(f"segments: starts {starts.dtype} {tuple(starts.shape)}, adapters {ids.dtype} "
-                         f"{tuple(ids.shape)}")
-    if any(t is not None and t.device != x.device for t in (a, b, scale, starts, ids)):
+def _check(x, n, a, b, scale, starts, ids):
+    """(K, adapters, rank, segments) of a call whose tensors fit each other."""
+    sa, sb, k, dtype, device = a.shape, b.shape, x.shape[-1], x.dtype, x.device
+    if len(sa) != 3 or len(sb) != 3 or sa[0] != sb[0] or sa[1] != sb[2] or not sa[0] * sa[1] * sa[2]:
+        raise ValueError(f"adapters a {tuple(sa)}, b {tuple(sb)}")
+    if sa[2] != k or sb[1] != n:
+        raise ValueError(f"adapters a {tuple(sa)}, b {tuple(sb)} for {k} -> {n}")
+    if a.dtype != dtype or b.dtype != dtype or not dtype.is_floating_point:
+        raise ValueError(f"dtypes x {dtype}, a {a.dtype}, b {b.dtype}")
+    if scale is not None and (scale.shape != sa[:1] or scale.dtype != torch.float32):
+        raise ValueError(f"scale {scale.dtype} {tuple(scale.shape)} of {sa[0]} adapters")
+    ss, si = starts.shape, ids.shape
+    if (len(ss) != 1 or len(si) != 1 or ss[0] != si[0] + 1 or starts.dtype not in _INDEX or ids.dtype not in _INDEX):
+        raise ValueError(f"segments: starts {starts.dtype} {tuple(ss)}, adapters {ids.dtype} {tuple(si)}")
+    if (a.device != device or b.device != device or starts.device != device or ids.device != device
+            or (scale is not None and scale.device != device)):
         raise ValueError("adapter inputs on different devices")
+    return k, sa[0], sa[1], si[0]
 
 
-def _kernel_ok(x, n, a) -> bool:
-    return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and a.shape[1] % 8 == 0 and a.shape[1] <= 128
-            and x.shape[-1] % 8 == 0 and n % 8 == 0 and a.shape[0] <= 2000)
+def _kernel_ok(x, n, k, rank, adapters) -> bool:
+    return (x.is_cuda and (x.dtype == torch.bfloat16 or x.dtype == torch.float16) and rank % 8 == 0 and rank <= 128
+            and k % 8 == 0 and n % 8 == 0 and adapters <= 2000)
 
 
 def _i32(t: torch.Tensor, most: int) -> torch.Tensor:
     if t.dtype != torch.int32:
         t = t.clamp(-1, most).to(torch.int32)
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _packed(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _torch_rows(x, a, starts, ids, scale):
@@ -108,18 +112,19 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     """y + scale (x a^T) b^T row by row, into `out` (which may be y) or a new
     tensor; with `save_low` also the rows' scale (x a^T), which
     `lora_backward` reads."""
-    _check(x, y.shape[-1], a, b, scale, segment_starts, segment_adapters)
-    if y.shape[:-1] != x.shape[:-1] or y.dtype != x.dtype or y.device != x.device:
-        raise ValueError(f"y {y.dtype} {tuple(y.shape)} for x {x.dtype} {tuple(x.shape)}")
+    shape = y.shape
+    n = shape[-1]
+    k, adapters, rank, segments = _check(x, n, a, b, scale, segment_starts, segment_adapters)
+    if shape[:-1] != x.shape[:-1] or y.dtype != x.dtype or y.device != x.device:
+        raise ValueError(f"y {y.dtype} {tuple(shape)} for x {x.dtype} {tuple(x.shape)}")
     if out is not None and (out.shape != y.shape or out.dtype != y.dtype or out.device != y.device
                             or not out.is_contiguous()):
         raise ValueError(f"out {out.dtype} {tuple(out.shape)} for y {y.dtype} {tuple(y.shape)}, contiguous")
-    n, k, rank = y.shape[-1], x.shape[-1], a.shape[1]
-    rows = x.numel() // k if k else 0
-    if rows == 0 or segment_adapters.shape[0] == 0:
+    rows = x.numel() // k
+    if rows == 0 or segments == 0:
         r = y.clone(memory_format=torch.contiguous_format) if out is None else out if out is y else out.copy_(y)
         return (r, torch.zeros((rows, rank), device=x.device, dtype=torch.float32)) if save_low else r
-    if not _kernel_ok(x, n, a) or (out is not None and out.data_ptr() % 16):
+    if not _kernel_ok(x, n, k, rank, adapters) or (out is not None and out.data_ptr() % 16):
         _fallback("lora_add", y, x)
         x2 = x.reshape(-1, k)
         keep, s = _torch_rows(x2, a, segment_starts, segment_adapters, scale)
@@ -129,18 +134,18 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         r = r if out is None else out.copy_(r)
         return (r, low.reshape(rows, -1, rank).sum(1)) if save_low else r
     if out is None:
-        out = torch.empty(y.shape, device=y.device, dtype=y.dtype)
+        out = torch.empty(shape, device=y.device, dtype=y.dtype)
     x2, xs = rows_layout(x)
     y2, ys = rows_layout(y)
     low = torch.empty((rows, rank), device=x.device, dtype=torch.float32) if save_low else None
     a, b = _packed(a), _packed(b)
-    scale = None if scale is None else scale.contiguous()
-    starts, ids = _i32(segment_starts, rows), _i32(segment_adapters, a.shape[0])
-    size = bytes_on(x, "oga_lora_add_workspace_bytes", rows, k, rank, ids.shape[0])
+    scale = scale if scale is None or scale.is_contiguous() else scale.contiguous()
+    starts, ids = _i32(segment_starts, rows), _i32(segment_adapters, adapters)
+    size = bytes_on(x, "oga_lora_add_workspace_bytes", rows, k, rank, segments)
     ws = torch.empty((size,), device=x.device, dtype=torch.uint8)
     _hip("lora_add")
     call_on(x, "oga_lora_add", _xdt(x), y2.data_ptr(), ys, x2.data_ptr(), xs, a.data_ptr(), b.data_ptr(),
-            None if scale is None else scale.data_ptr(), starts.data_ptr(), ids.data_ptr(), ids.shape[0], a.shape[0],
+            None if scale is None else scale.data_ptr(), starts.data_ptr(), ids.data_ptr(), segments, adapters,
             None if low is None else low.data_ptr(), out.data_ptr(), n, rows, k, n, rank, ws.data_ptr(), size)
     return (out, low) if save_low else out
 
@@ -149,16 +154,16 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, low: torch.Tensor, a: torch
                   scale: torch.Tensor | None, segment_starts: torch.Tensor, segment_adapters: torch.Tensor):
     """dx, da, db of `lora_add` with these inputs from its output's gradient
     and the `low` it saved (y's gradient is dy)."""
-    n, k, rank = dy.shape[-1], x.shape[-1], a.shape[1]
-    _check(x, n, a, b, scale, segment_starts, segment_adapters)
+    n = dy.shape[-1]
+    k, adapters, rank, segments = _check(x, n, a, b, scale, segment_starts, segment_adapters)
     if dy.shape[:-1] != x.shape[:-1] or dy.dtype != x.dtype or dy.device != x.device:
         raise ValueError(f"dy {dy.dtype} {tuple(dy.shape)} for x {x.dtype} {tuple(x.shape)}")
-    rows = x.numel() // k if k else 0
+    rows = x.numel() // k
     if low.shape != (rows, rank) or low.device != x.device or not low.is_floating_point():
         raise ValueError(f"low {low.dtype} {tuple(low.shape)} of {rows} rows, rank {rank}")
-    if rows == 0 or segment_adapters.shape[0] == 0:
+    if rows == 0 or segments == 0:
         return torch.zeros(x.shape, device=x.device, dtype=x.dtype), torch.zeros_like(a), torch.zeros_like(b)
-    if not _kernel_ok(x, n, a) or low.dtype != torch.float32:
+    if not _kernel_ok(x, n, k, rank, adapters) or low.dtype != torch.float32:
         _fallback("lora_backward", dy, x)
         x2, dy2 = x.reshape(-1, k), dy.reshape(-1, n)
         keep, s = _torch_rows(x2, a, segment_starts, segment_adapters, scale)
@@ -174,15 +179,15 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, low: torch.Tensor, a: torch
     x2, xs = rows_layout(x)
     dy2, dys = rows_layout(dy)
     low, a, b = _packed(low), _packed(a), _packed(b)
-    scale = None if scale is None else scale.contiguous()
-    starts, ids = _i32(segment_starts, rows), _i32(segment_adapters, a.shape[0])
+    scale = scale if scale is None or scale.is_contiguous() else scale.contiguous()
+    starts, ids = _i32(segment_starts, rows), _i32(segment_adapters, adapters)
     da, db = torch.empty_like(a), torch.empty_like(b)
-    size = bytes_on(x, "oga_lora_bwd_workspace_bytes", rows, k, n, rank, a.shape[0], ids.shape[0])
+    size = bytes_on(x, "oga_lora_bwd_workspace_bytes", rows, k, n, rank, adapters, segments)
     ws = torch.empty((size,), device=x.device, dtype=torch.uint8)
     _hip("lora_backward")
     call_on(x, "oga_lora_bwd", _xdt(x), dy2.data_ptr(), dys, x2.data_ptr(), xs, low.data_ptr(), a.data_ptr(),
             b.data_ptr(), None if scale is None else scale.data_ptr(), starts.data_ptr(), ids.data_ptr(),
-            ids.shape[0], a.shape[0], dx.data_ptr(), k, da.data_ptr(), db.data_ptr(), rows, k, n, rank, ws.data_ptr(),
+            segments, adapters, dx.data_ptr(), k, da.data_ptr(), db.data_ptr(), rows, k, n, rank, ws.data_ptr(),
             size)
     return dx, da, db
 
