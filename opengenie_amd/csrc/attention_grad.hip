@@ -35,7 +35,7 @@ struct AttnGradArgs {
   uint16_t *o, *dq, *dk, *dv;
   int64_t q_s[3], k_s[3], v_s[3], do_s[3], o_s[3], dq_s[3], dk_s[3], dv_s[3];  // (batch, token, head); unit along D
   float* lse;          // [B, H, Nq]
-  float* ld;           // [B, H, ceil(Nq / 64)][64 lse2 | 64 Delta] (backward)
+  float* ld;           // [B, H, ceil(Nq / 64)][64 lse2 | 64 -Delta] (backward)
   float* part;         // what the parts of split blocks leave, float32
   float* part_ml;      // k_attn_lse: their running maxima and sums
   const int32_t* k_lens;
@@ -181,23 +181,57 @@ OGA_DEVICE f32x4 mfma16(const bf16x8& a, const bf16x8& b, const f32x4& c) {
 
 // LDS-DMA of a 64-row tile by W waves: instruction i of wave w fills 1 KiB.
 // Rows past the last one (`rows` of them exist) read the last one again.
-// A source is a uniform base and a 32-bit offset made anew for each tile from
-// the lane number: kept over the loop, the offsets would be the registers that
-// k_attn_dkv does not have.
-template <int D, int W, bool S16>
+// A source is a uniform base and a 32-bit offset per lane. HOLD 2 keeps the two
+// operands' offsets over the loop (4 registers). k_attn_dkv at D 128 has none
+// to spare and makes them anew for each tile from the lane number: HOLD 1 once
+// where the operands' row strides are equal, 0 (causal) for each operand, as
+// even that costs spills.
+template <int D, int W, bool S16, int HOLD>
 struct TileDma {
+  static constexpr bool KEEP = HOLD == 2;
   static constexpr int kCh = D / 8, kRpi = 64 / kCh, kDI = kGT / kRpi / W;
   static_assert(kDI >= 1, "waves");
-  static OGA_DEVICE void send(const uint16_t* base, uint32_t row_stride, int rows, char* lds, int wv, int lane) {
-    asm volatile("" : "+v"(lane));
+  struct Off {
+    uint32_t o[kDI];
+  };
+  Off full[KEEP ? 2 : 1];
+  static OGA_DEVICE void offsets(Off& f, uint32_t row_stride, int rows, int wv, int lane) {
 #pragma unroll
     for (int i = 0; i < kDI; ++i) {
-      const int row = (wv * kDI + i) * kRpi + lane / kCh;
+      int row = (wv * kDI + i) * kRpi + lane / kCh;
       const int chunk = (lane % kCh) ^ (S16 ? sw16<D>(row) : sw32<D>(row));
-      const uint32_t off = __umul24((uint32_t)min(row, rows - 1), row_stride) * 2 + chunk * 16;
-      __builtin_amdgcn_global_load_lds((const void*)((const char*)base + off),
-                                       (lds_void*)(lds + (wv * kDI + i) * 1024), 16, 0, 0);
+      if (HOLD == 0 || rows < kGT) row = min(row, rows - 1);
+      f.o[i] = __umul24((uint32_t)row, row_stride) * 2 + chunk * 16;
     }
+  }
+  static OGA_DEVICE void send(const uint16_t* base, const Off& f, char* lds, int wv) {
+#pragma unroll
+    for (int i = 0; i < kDI; ++i)
+      __builtin_amdgcn_global_load_lds((const void*)((const char*)base + f.o[i]),
+                                       (lds_void*)(lds + (wv * kDI + i) * 1024), 16, 0, 0);
+  }
+  OGA_DEVICE void init(uint32_t s0, uint32_t s1, int wv, int lane) {
+    if constexpr (KEEP) {
+      offsets(full[0], s0, kGT, wv, lane);
+      offsets(full[1], s1, kGT, wv, lane);
+    }
+  }
+  // The same `rows` rows of both operands into the tile pair at lds.
+  OGA_DEVICE void pair(const uint16_t* b0, uint32_t s0, const uint16_t* b1, uint32_t s1, int rows, char* lds, int wv,
+                       int lane) const {
+    constexpr int kTile = kGT * D * 2;
+    if (KEEP && rows >= kGT) {
+      send(b0, full[0], lds, wv);
+      send(b1, full[KEEP ? 1 : 0], lds + kTile, wv);
+      return;
+    }
+    asm volatile("" : "+v"(lane));
+    Off f;
+    offsets(f, s0, rows, wv, lane);
+    send(b0, f, lds, wv);
+    if (HOLD == 0) asm volatile("" : "+v"(lane));
+    if (HOLD == 0 || s1 != s0) offsets(f, s1, rows, wv, lane);
+    send(b1, f, lds + kTile, wv);
   }
 };
 
@@ -228,7 +262,7 @@ template <int D, int W, int BUFS, bool CAUSAL>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void k_attn_lse(
     AttnGradArgs a) {
   constexpr int kTile = kGT * D * 2, kPair = 2 * kTile, NS = D / 16, ND = D / 32;
-  typedef TileDma<D, W, false> Dma;
+  typedef TileDma<D, W, false, 2> Dma;
   __shared__ uint4 smem[BUFS * kPair / 16];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -251,11 +285,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
   const uint16_t* kb = a.k + b * a.k_s[0] + (int64_t)hk * a.k_s[2];
   const uint16_t* vb = a.v + b * a.v_s[0] + (int64_t)hk * a.v_s[2];
   char* const lds = (char*)smem;
+  Dma tiles;
+  tiles.init((uint32_t)a.k_s[1], (uint32_t)a.v_s[1], wv, lane);
   auto dma = [&](int st, int slot) {
     const int64_t key0 = (int64_t)st * kGT;
-    const int rows = (int)min((int64_t)kGT, nkb - key0);
-    Dma::send(kb + key0 * a.k_s[1], (uint32_t)a.k_s[1], rows, lds + slot * kPair, wv, lane);
-    Dma::send(vb + key0 * a.v_s[1], (uint32_t)a.v_s[1], rows, lds + slot * kPair + kTile, wv, lane);
+    tiles.pair(kb + key0 * a.k_s[1], (uint32_t)a.k_s[1], vb + key0 * a.v_s[1], (uint32_t)a.v_s[1],
+               (int)min((int64_t)kGT, nkb - key0), lds + slot * kPair, wv, lane);
   };
   if (st1 > st0) {  // (uniform over the workgroup) in flight under the loads below
     dma(st0, 0);
@@ -496,7 +531,7 @@ template <int D, int W, int BUFS, bool CAUSAL>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void k_attn_dq(
     AttnGradArgs a) {
   constexpr int kTile = kGT * D * 2, kPair = 2 * kTile, NS = D / 32, ND = D / 16;
-  typedef TileDma<D, W, true> Dma;
+  typedef TileDma<D, W, true, 2> Dma;
   __shared__ uint4 smem[BUFS * kPair / 16];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -519,11 +554,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
   const uint16_t* kb = a.k + b * a.k_s[0] + (int64_t)hk * a.k_s[2];
   const uint16_t* vb = a.v + b * a.v_s[0] + (int64_t)hk * a.v_s[2];
   char* const lds = (char*)smem;
+  Dma tiles;
+  tiles.init((uint32_t)a.k_s[1], (uint32_t)a.v_s[1], wv, lane);
   auto dma = [&](int st, int slot) {
     const int64_t key0 = (int64_t)st * kGT;
-    const int rows = (int)min((int64_t)kGT, nkb - key0);
-    Dma::send(kb + key0 * a.k_s[1], (uint32_t)a.k_s[1], rows, lds + slot * kPair, wv, lane);
-    Dma::send(vb + key0 * a.v_s[1], (uint32_t)a.v_s[1], rows, lds + slot * kPair + kTile, wv, lane);
+    tiles.pair(kb + key0 * a.k_s[1], (uint32_t)a.k_s[1], vb + key0 * a.v_s[1], (uint32_t)a.v_s[1],
+               (int)min((int64_t)kGT, nkb - key0), lds + slot * kPair, wv, lane);
   };
   if (st1 > st0) {  // (uniform over the workgroup) in flight under the loads below
     dma(st0, 0);
@@ -563,7 +599,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
     if (kg == 0 && row < nqt * kGT && unit.part <= 0) {
       float* t = a.ld + (bh * nqt + row / kGT) * 128 + row % kGT;
       t[0] = lse2[i];
-      t[64] = row < a.nq ? delta[i] : 0.0f;
+      t[64] = row < a.nq ? -delta[i] : 0.0f;
     }
   }
   f32x4 acc[ND][2];
@@ -577,10 +613,20 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
   const int a4 = lane & 3, j4 = (lane & 15) >> 2;
   const uint32_t ta = lds0 + (4 * kg + j4) * (2 * D) + (((a4 >> 1) ^ sw16<D>(4 * kg + j4)) << 4) + (a4 & 1) * 8;
 
+  uint32_t ra4[NS], ta8[ND];
+#pragma unroll
+  for (int x = 0; x < NS; ++x) ra4[x] = ra ^ (x << 6);
+#pragma unroll
+  for (int x = 0; x < ND; ++x) ta8[x] = ta ^ (x << 5);
   auto step = [&](uint32_t base, int slot2, int st) {
+    uint32_t rs[NS], ts[ND];
     ring_wait<BUFS == 3 ? 2 * Dma::kDI : 0>();
     if (BUFS == 3 || st + 1 < st1) dma(min(st + BUFS - 1, st1 - 1), slot2);
     if (q0 >= a.nq || (CAUSAL && (int64_t)st * kGT > q0 + 31 + shift)) return;
+#pragma unroll
+    for (int x = 0; x < NS; ++x) rs[x] = ra4[x] + base;
+#pragma unroll
+    for (int x = 0; x < ND; ++x) ts[x] = ta8[x] + base;
     const int64_t key0 = (int64_t)st * kGT;
     const bool edge = CAUSAL ? key0 + kGT > min(nkb, q0 + shift + 1) : key0 + kGT > nkb;
     auto half = [&](auto j_c) {  // keys 32 j .. + 31 of the tile
@@ -588,19 +634,21 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
       uint32_t ds[2][4];  // dS^T, B operand of dq: query block i
       auto block = [&](auto u_c) {  // keys 16 u .. + 15 of these
         constexpr int U = decltype(u_c)::value;
-        const uint32_t r0 = here(ra, base);
         f32x4 s[2], g[2];
         bf16x8 kf[NS], vf[NS];
 #pragma unroll
-        for (int x = 0; x < NS; ++x) kf[x] = rd_b128<OFF + 16 * 2 * D * U>(r0 ^ (x << 6));
+        for (int x = 0; x < NS; ++x) kf[x] = rd_b128<OFF + 16 * 2 * D * U>(rs[x]);
 #pragma unroll
-        for (int x = 0; x < NS; ++x) vf[x] = rd_b128<OFF + 16 * 2 * D * U + kTile>(r0 ^ (x << 6));
+        for (int x = 0; x < NS; ++x) vf[x] = rd_b128<OFF + 16 * 2 * D * U + kTile>(rs[x]);
         if constexpr (NS == 4)
           GRAD_LGKM(4, "+v"(kf[0]), "+v"(kf[1]), "+v"(kf[2]), "+v"(kf[3]));
         else
           GRAD_LGKM(2, "+v"(kf[0]), "+v"(kf[1]));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) s[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, g[i] = s[i];
+        for (int i = 0; i < 2; ++i) {  // dP - Delta from the product's start value
+          s[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          g[i] = f32x4{-delta[i], -delta[i], -delta[i], -delta[i]};
+        }
 #pragma unroll
         for (int x = 0; x < NS; ++x)
 #pragma unroll
@@ -629,7 +677,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], a.scale_log2, -lse2[i]));
-            d[r] = p * (g[i][r] - delta[i]);
+            d[r] = p * g[i][r];
           }
           ds[i][2 * U] = pack_bf16(d[0], d[1]);
           ds[i][2 * U + 1] = pack_bf16(d[2], d[3]);
@@ -645,12 +693,11 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
       }
 #pragma unroll
       for (int d = 0; d < ND; d += 4) {
-        const uint32_t w0 = here(ta, base);
         u32x2 t[8];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          t[2 * x] = rd_tr16<OFF>(w0 ^ ((d + x) << 5));
-          t[2 * x + 1] = rd_tr16<OFF + 16 * 2 * D>(w0 ^ ((d + x) << 5));
+          t[2 * x] = rd_tr16<OFF>(ts[d + x]);
+          t[2 * x + 1] = rd_tr16<OFF + 16 * 2 * D>(ts[d + x]);
         }
         GRAD_LGKM(0, "+v"(t[0]), "+v"(t[1]), "+v"(t[2]), "+v"(t[3]), "+v"(t[4]), "+v"(t[5]), "+v"(t[6]), "+v"(t[7]));
 #pragma unroll
@@ -704,7 +751,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
     AttnGradArgs a) {
   constexpr int kTile = kGT * D * 2, kPair = 2 * kTile + 512, NS = D / 32, ND = D / 16;
   constexpr int KB = 2, kKeys = 32 * W;
-  typedef TileDma<D, W, true> Dma;
+  typedef TileDma<D, W, true, D == 64 ? 2 : CAUSAL ? 0 : 1> Dma;
   __shared__ uint4 smem[BUFS * kPair / 16];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -751,6 +798,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
     const uint16_t* gbase = a.dout + b * a.do_s[0] + (int64_t)hk * a.group * a.do_s[2];
     const float* lbase = a.ld + (b * a.heads + (int64_t)hk * a.group) * nqt * 128;
     char* const lds = (char*)smem;
+    Dma tiles;
+    tiles.init((uint32_t)a.q_s[1], (uint32_t)a.do_s[1], wv, lane);
     // The next step to send: its head of the group and query tile (the last
     // one again past the end).
     int send_s = s0, send_g = s0 / per, send_t = t0 + s0 % per;
@@ -763,8 +812,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
       const int64_t q0 = (int64_t)t * kGT;
       const int rows = (int)min((int64_t)kGT, a.nq - q0);
       char* const at = lds + slot * kPair;
-      Dma::send(qbase + g * a.q_s[2] + q0 * a.q_s[1], (uint32_t)a.q_s[1], rows, at, wv, lane);
-      Dma::send(gbase + g * a.do_s[2] + q0 * a.do_s[1], (uint32_t)a.do_s[1], rows, at + kTile, wv, lane);
+      tiles.pair(qbase + g * a.q_s[2] + q0 * a.q_s[1], (uint32_t)a.q_s[1], gbase + g * a.do_s[2] + q0 * a.do_s[1],
+                 (uint32_t)a.do_s[1], rows, at, wv, lane);
       // lse2 and Delta, 256 bytes each: even waves the one, odd waves the other
       int l = lane;
       asm volatile("" : "+v"(l));
@@ -791,15 +840,23 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
           constexpr int OQ = OFF + 16 * 2 * D * U, OG = OQ + kTile, OL = (32 * J + 16 * U) * 4;
           f32x4 s[KB], g[KB];
 #pragma unroll
-          for (int i = 0; i < KB; ++i) s[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f}, g[i] = s[i];
+          for (int i = 0; i < KB; ++i) s[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
           // two pairs of fragments in flight, each read under the other's MFMAs
-          bf16x8 x0, x1, y0, y1;
+          bf16x8 x0, x1, y0, y1, dr;
           auto mul = [&](f32x4(&c)[KB], const bf16x8& u, const bf16x8& v, const bf16x8(&w)[KB][NS], auto n_c) {
             constexpr int N = decltype(n_c)::value;
 #pragma unroll
             for (int i = 0; i < KB; ++i) c[i] = mfma16(u, w[i][N], c[i]);
 #pragma unroll
             for (int i = 0; i < KB; ++i) c[i] = mfma16(v, w[i][N + 1], c[i]);
+          };
+          const uint32_t l0 = (here(lane, 0) & ~15u) + lds0 + 2 * kTile + base;  // 16 kg
+          // dP - Delta from the product's start value (subtracted after it
+          // where -Delta would be one register too many)
+          constexpr bool kStart = D == 64 || !CAUSAL;
+          auto start = [&] {
+#pragma unroll
+            for (int i = 0; i < KB; ++i) g[i] = kStart ? __builtin_bit_cast(f32x4, dr) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
           };
           x0 = rd_b128<OQ>(r0);
           x1 = rd_b128<OQ>(r0 ^ 64);
@@ -808,37 +865,50 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
             y1 = rd_b128<OQ>(r0 ^ 192);
             GRAD_LGKM(2, "+v"(x0), "+v"(x1));
             mul(s, x0, x1, kf, IC<0>{});
+            if constexpr (kStart) dr = rd_b128<OL + 256>(l0);
             x0 = rd_b128<OG>(r0);
             x1 = rd_b128<OG>(r0 ^ 64);
-            GRAD_LGKM(2, "+v"(y0), "+v"(y1));
+            if constexpr (kStart)
+              GRAD_LGKM(3, "+v"(y0), "+v"(y1));
+            else
+              GRAD_LGKM(2, "+v"(y0), "+v"(y1));
             mul(s, y0, y1, kf, IC<2 % NS>{});
             y0 = rd_b128<OG>(r0 ^ 128);
             y1 = rd_b128<OG>(r0 ^ 192);
-            GRAD_LGKM(2, "+v"(x0), "+v"(x1));
+            if constexpr (kStart)
+              GRAD_LGKM(2, "+v"(x0), "+v"(x1), "+v"(dr));
+            else
+              GRAD_LGKM(2, "+v"(x0), "+v"(x1));
+            start();
             mul(g, x0, x1, vf, IC<0>{});
-            const uint32_t l0 = (here(lane, 0) & ~15u) + lds0 + 2 * kTile + base;  // 16 kg
             x0 = rd_b128<OL>(l0);
-            x1 = rd_b128<OL + 256>(l0);
-            GRAD_LGKM(2, "+v"(y0), "+v"(y1));
+            if constexpr (!kStart) dr = rd_b128<OL + 256>(l0);
+            if constexpr (kStart)
+              GRAD_LGKM(1, "+v"(y0), "+v"(y1));
+            else
+              GRAD_LGKM(2, "+v"(y0), "+v"(y1));
             mul(g, y0, y1, vf, IC<2 % NS>{});
           } else {
+            dr = rd_b128<OL + 256>(l0);
             y0 = rd_b128<OG>(r0);
             y1 = rd_b128<OG>(r0 ^ 64);
-            GRAD_LGKM(2, "+v"(x0), "+v"(x1));
+            GRAD_LGKM(3, "+v"(x0), "+v"(x1));
             mul(s, x0, x1, kf, IC<0>{});
-            const uint32_t l0 = (here(lane, 0) & ~15u) + lds0 + 2 * kTile + base;  // 16 kg
             x0 = rd_b128<OL>(l0);
-            x1 = rd_b128<OL + 256>(l0);
-            GRAD_LGKM(2, "+v"(y0), "+v"(y1));
+            GRAD_LGKM(1, "+v"(y0), "+v"(y1), "+v"(dr));
+            start();
             mul(g, y0, y1, vf, IC<0>{});
           }
-          GRAD_LGKM(0, "+v"(x0), "+v"(x1));
-          const f32x4 lse2 = __builtin_bit_cast(f32x4, x0), delta = __builtin_bit_cast(f32x4, x1);
-          if constexpr (CAUSAL) {
+          if constexpr (kStart)
+            GRAD_LGKM(0, "+v"(x0));
+          else
+            GRAD_LGKM(0, "+v"(x0), "+v"(dr));
+          const f32x4 lse2 = __builtin_bit_cast(f32x4, x0);
+          // (D 128 compares in every tile: behind a uniform branch the scores
+          // cost more registers than there are)
+          if (CAUSAL && (D == 128 || first + 16 * KB - 1 > 0)) {
 #pragma unroll
             for (int i = 0; i < KB; ++i) {
-              // compared in every tile: behind a uniform branch the scores cost
-              // more registers than there are
               const int l = (int)here(lane, 0);
               const int low = first + 16 * i + (l & 15) - 4 * (l >> 4) - 32 * J - 16 * U;
 #pragma unroll
@@ -852,7 +922,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], a.scale_log2, -lse2[r]));
-              d[r] = p[r] * (g[i][r] - delta[r]);
+              d[r] = p[r] * (kStart ? g[i][r] : g[i][r] + __builtin_bit_cast(f32x4, dr)[r]);
             }
             pp[i][2 * U] = pack_bf16(p[0], p[1]);
             pp[i][2 * U + 1] = pack_bf16(p[2], p[3]);
