@@ -27,7 +27,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kGT = 64;    // rows of a tile
+constexpr int kGT = 64;        // rows of a tile
+constexpr int kMaxParts = 16;  // of a split block
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct AttnGradArgs {
@@ -488,26 +489,29 @@ __global__ __launch_bounds__(256) void k_attn_lse_join(AttnGradArgs a) {
   if (qi >= a.nq) return;
   const int c = threadIdx.x % kLpr;
   const int64_t first = blk * a.ksplit * ROWS + row;
-  float m = -INFINITY;
-#pragma unroll 4
-  for (int p = 0; p < a.ksplit; ++p) m = __builtin_fmaxf(m, a.part_ml[2 * (first + p * ROWS)]);
-  const float nm = m == -INFINITY ? 0.0f : -m;
-  float l = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int p0 = 0; p0 < a.ksplit; p0 += 4) {  // four parts' loads in flight
-    float2 ml[4];
-    float4 u[4], v[4];
+  float2 ml[kMaxParts];  // with the first parts' loads behind them, before any is used
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int64_t at = first + min(p0 + e, a.ksplit - 1) * ROWS;
-      const float* f = a.part + at * D + 8 * c;
-      ml[e] = *(const float2*)(a.part_ml + 2 * at);
+  for (int p = 0; p < kMaxParts; ++p) ml[p] = *(const float2*)(a.part_ml + 2 * (first + min(p, a.ksplit - 1) * ROWS));
+  float m = -INFINITY, nm = 0.0f, l = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+  for (int p0 = 0; p0 < kMaxParts; p0 += 8) {
+    if (p0 >= a.ksplit) break;
+    float4 u[8], v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float* f = a.part + (first + min(p0 + e, a.ksplit - 1) * ROWS) * D + 8 * c;
       u[e] = *(const float4*)f, v[e] = *(const float4*)(f + 4);
     }
+    if (p0 == 0) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+      for (int p = 0; p < kMaxParts; ++p) m = __builtin_fmaxf(m, ml[p].x);  // a part read twice changes nothing
+      nm = m == -INFINITY ? 0.0f : -m;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
       if (p0 + e >= a.ksplit) break;
-      const float w = __builtin_amdgcn_exp2f(ml[e].x + nm);
-      l = fmaf(w, ml[e].y, l);
+      const float w = __builtin_amdgcn_exp2f(ml[p0 + e].x + nm);
+      l = fmaf(w, ml[p0 + e].y, l);
       o[0] = fmaf(w, u[e].x, o[0]), o[1] = fmaf(w, u[e].y, o[1]), o[2] = fmaf(w, u[e].z, o[2]), o[3] = fmaf(w, u[e].w, o[3]);
       o[4] = fmaf(w, v[e].x, o[4]), o[5] = fmaf(w, v[e].y, o[5]), o[6] = fmaf(w, v[e].z, o[6]), o[7] = fmaf(w, v[e].w, o[7]);
     }
@@ -1047,15 +1051,15 @@ __global__ __launch_bounds__(256) void k_attn_grad_join(GradJoins a) {
   const float* f = j.part + (blk * j.ksplit * j.rows + row) * width + c;
   float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   const int64_t step = (int64_t)j.rows * width;
-  for (int p0 = 0; p0 < j.ksplit; p0 += 4) {  // four parts' loads in flight
-    float4 u[4], v[4];
+  for (int p0 = 0; p0 < j.ksplit; p0 += 8) {  // eight parts' loads in flight
+    float4 u[8], v[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 8; ++e) {
       const float* g = f + min(p0 + e, j.ksplit - 1) * step;
       u[e] = *(const float4*)g, v[e] = *(const float4*)(g + 4);
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 8; ++e) {
       if (p0 + e >= j.ksplit) break;
       s[0] += u[e].x, s[1] += u[e].y, s[2] += u[e].z, s[3] += u[e].w;
       s[4] += v[e].x, s[5] += v[e].y, s[6] += v[e].z, s[7] += v[e].w;
@@ -1090,7 +1094,7 @@ static GradPlan grad_plan(int64_t blocks, int64_t steps, int64_t slots, double s
   const int64_t whole = equal ? blocks / slots * slots : 0, rest = blocks - whole;
   if (!rest || steps < 2) return best;
   double least = 1e30;
-  for (int k = 1; k <= 16 && k <= steps; ++k) {
+  for (int k = 1; k <= kMaxParts && k <= steps; ++k) {
     const double part = (double)((steps + k - 1) / k) * step_us + (k > 1 ? fixed_us : 0.0);
     double us = equal ? (double)((rest * k + slots - 1) / slots) * part
                       : max(part, (double)(rest * k) / slots * (fill * part) + 0.5 * part);
