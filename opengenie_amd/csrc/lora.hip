@@ -569,16 +569,20 @@ __global__ __launch_bounds__(256) void k_lora_join(JoinArgs a) {
 // -------------------------------------------------------------------- host
 // Blocks of 16 rows in a tile: more where segments are long and each fragment
 // of the weights serves more rows, one where they are single tokens.
-static int row_blocks(const Segments& g, int most) {
-  const int64_t mean = g.rows / g.count;
+static int row_blocks(int64_t rows, int64_t segments, int most) {
+  const int64_t mean = rows / segments;
   return mean >= 48 ? most : mean >= 16 ? min(most, 2) : 1;
 }
 
-// Parts of the long axis: with three workgroups a CU at a time, the number
-// whose rounds times a part's length is least (each wave with two chunks or
-// more).
-static int shrink_parts(int64_t rows, int64_t segments, int64_t k) {
-  const int64_t pairs = seg_pairs(rows, segments, rows / segments >= 16 ? 32 : 16), slots = 3 * (int64_t)cu_count();
+// (Rank 128 holds its weights' fragments for 32 rows at most.)
+static int shrink_tiles(int64_t rank) { return rank > 64 ? 2 : 4; }
+
+// Parts of the long axis: with two (64-row tiles) or three workgroups a CU at
+// a time, the number whose rounds times a part's length is least (each wave
+// with two chunks or more).
+static int shrink_parts(int64_t rows, int64_t segments, int64_t k, int64_t rank) {
+  const int tb = row_blocks(rows, segments, shrink_tiles(rank));
+  const int64_t pairs = seg_pairs(rows, segments, 16 * tb), slots = (tb == 4 ? 2 : 3) * (int64_t)cu_count();
   const int64_t most = min((k + 63) / 64 / (2 * kShrinkWaves), (int64_t)8);
   int best = 1;
   double least = 1e30;
@@ -591,12 +595,15 @@ static int shrink_parts(int64_t rows, int64_t segments, int64_t k) {
 
 template <int XDT, int RB>
 static void shrink_launch(const ShrinkArgs& a, int parts, hipStream_t s) {
-  constexpr int TB = RB >= 8 ? 1 : 2;
-  const dim3 block(64 * kShrinkWaves);
-  if (row_blocks(a.g, TB) == TB)
-    k_lora_shrink<XDT, RB, TB><<<dim3((unsigned)seg_pairs(a.g.rows, a.g.count, 16 * TB), parts), block, 0, s>>>(a);
+  constexpr int most = RB >= 8 ? 2 : 4;
+  const int tb = row_blocks(a.g.rows, a.g.count, most);
+  const dim3 grid((unsigned)seg_pairs(a.g.rows, a.g.count, 16 * tb), parts), block(64 * kShrinkWaves);
+  if (tb == 4)
+    k_lora_shrink<XDT, RB, most><<<grid, block, 0, s>>>(a);
+  else if (tb == 2)
+    k_lora_shrink<XDT, RB, 2><<<grid, block, 0, s>>>(a);
   else
-    k_lora_shrink<XDT, RB, 1><<<dim3((unsigned)seg_pairs(a.g.rows, a.g.count, 16), parts), block, 0, s>>>(a);
+    k_lora_shrink<XDT, RB, 1><<<grid, block, 0, s>>>(a);
 }
 template <int XDT>
 static void shrink(const ShrinkArgs& a, int parts, hipStream_t s) {
@@ -619,7 +626,7 @@ static void expand_launch(ExpandArgs a, hipStream_t s) {
 template <int XDT, int KS>
 static void expand_rows(const ExpandArgs& a, hipStream_t s) {
   constexpr int most = KS >= 4 ? 2 : 4;
-  const int tb = row_blocks(a.g, most);
+  const int tb = row_blocks(a.g.rows, a.g.count, most);
   if (tb == 4)
     expand_launch<XDT, KS, most, 8>(a, s);
   else if (tb == 2)
@@ -688,7 +695,7 @@ struct LoraBwdSpace {
 static LoraBwdSpace lora_bwd_space(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters,
                                    int64_t segments) {
   LoraBwdSpace w;
-  w.parts = shrink_parts(rows, segments, n);
+  w.parts = shrink_parts(rows, segments, n, rank);
   w.splits = wgrad_splits(rows, adapters, k, n, rank);
   w.dlow = align256(w.parts * rows * rank * 4);
   w.at = w.dlow + (w.parts > 1 ? align256(rows * rank * 4) : 0);
@@ -706,7 +713,7 @@ using namespace oga;
 
 extern "C" int64_t oga_lora_add_workspace_bytes(int64_t rows, int64_t k, int64_t rank, int64_t segments) {
   if (rows < 1 || k < 8 || rank < 8 || rank > 128 || segments < 1) return 0;
-  return align256(shrink_parts(rows, segments, k) * rows * rank * 4);
+  return align256(shrink_parts(rows, segments, k, rank) * rows * rank * 4);
 }
 
 extern "C" int oga_lora_add(int x_dtype, const void* y, int64_t y_stride, const void* x, int64_t x_stride,
@@ -722,7 +729,7 @@ extern "C" int oga_lora_add(int x_dtype, const void* y, int64_t y_stride, const 
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
     return fail("workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   const Segments g = {segment_starts, segment_adapters, (int)segments, (int)adapters, rows};
-  const int parts = shrink_parts(rows, segments, k);
+  const int parts = shrink_parts(rows, segments, k, rank);
   const ShrinkArgs sa = {g, x, x_stride, a, scale, (float*)workspace, k, (int)rank};
   const ExpandArgs ea = {g, (const float*)workspace, low, b, y, out, y_stride, out_stride, n, (int)rank, parts, 0};
   const hipStream_t s = (hipStream_t)stream;
