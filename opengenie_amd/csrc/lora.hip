@@ -83,17 +83,16 @@ struct Pair {
   int adapter;            // -1: none
 };
 
-// Pair number p for tiles of BM rows. Lanes test 64 segments at a time, each
+// Pair number p for tiles of bm rows. Lanes test 64 segments at a time, each
 // with its bounds and adapter loaded side by side (one memory latency).
-template <int BM>
-OGA_DEVICE Pair seg_pair(const Segments& g, int64_t p, int lane) {
+OGA_DEVICE Pair seg_pair(const Segments& g, int bm, int64_t p, int lane) {
   const int all = g.count + 2;
   int seg = 0, b0 = 0, b1 = 0, id = -1;
   for (int s0 = 0; s0 < all; s0 += 64) {
     const int s = s0 + lane;
     const int lo = (int)seg_bound(g, s), hi = (int)seg_bound(g, s + 1);  // (rows stay below 2^31)
     const int own = s >= 1 && s <= g.count ? g.ids[s - 1] : -1;
-    const unsigned long long m = __ballot(s < all && lo / BM + s <= p);
+    const unsigned long long m = __ballot(s < all && lo / bm + s <= p);
     if (!m) break;
     const int top = 63 - __builtin_clzll(m);
     seg = s0 + top;
@@ -103,9 +102,9 @@ OGA_DEVICE Pair seg_pair(const Segments& g, int64_t p, int lane) {
     if (top < 63) break;
   }
   Pair r;
-  r.tile0 = (p - seg) * BM;  // floor(b0 / BM) + j tiles down
+  r.tile0 = (p - seg) * bm;  // floor(b0 / bm) + j tiles down
   r.lo = max((int64_t)b0, r.tile0);
-  r.hi = min((int64_t)b1, r.tile0 + BM);
+  r.hi = min((int64_t)b1, r.tile0 + bm);
   r.adapter = id >= 0 && id < g.adapters ? id : -1;
   return r;
 }
@@ -134,7 +133,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void k_lora_shrink(ShrinkArgs a)
   __shared__ f32x4 red[kShrinkWaves][TB * RB][64];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const Pair p = seg_pair<16 * TB>(a.g, blockIdx.x, lane);
+  const Pair p = seg_pair(a.g, 16 * TB, blockIdx.x, lane);
   if (p.adapter < 0 || p.hi <= p.lo) return;  // (uniform over the workgroup)
   const int c = lane & 15, kg = 8 * (lane >> 4);
   const uint16_t* xr[TB];
@@ -250,51 +249,64 @@ struct ExpandArgs {
   int64_t ys, os;    // row strides
   int64_t n;
   int rank, parts;
+  int bm;
   uint32_t col_blocks;
 };
 
-// 16 TB rows x 128 columns per wave: operand A is low (16 rows, its two halves
-// as fragments in LDS, shared by the waves), operand B of product j the eight
-// columns' j-th, 8 (l % 16) + j for lane l, so that a lane ends with 8
-// consecutive columns of 4 rows and y moves in pieces of 256 bytes a row (16
-// rows x 64 bytes at a time, as the other orientation has it, moved 2.9 TB/s).
-template <int XDT, int KS, int TB, int W>
+// Up to bm rows x 128 columns per wave, 16 rows at a time: operand A is low
+// (16 rows, its two halves as fragments in LDS, shared by the waves), operand B
+// of product j the eight columns' j-th, 8 (l % 16) + j for lane l, so that a
+// lane ends with 8 consecutive columns of 4 rows and y moves in pieces of 256
+// bytes a row (16 rows x 64 bytes at a time, as the other orientation has it,
+// moved 2.9 TB/s). The weights' fragments stay in registers over the rows; y
+// runs RING x 16 rows ahead. Rows and columns past the end are offsets past the
+// end of a buffer resource, which loads give 0 for and stores drop: no branch
+// stands between the loads and the wait counts.
+template <int XDT, int KS, int RING, int W>
 __global__ __launch_bounds__(64 * W) void k_lora_expand(ExpandArgs a) {
-  __shared__ uint4 lows[TB][KS][2][64];
+  extern __shared__ uint4 lows[];  // [bm / 16, a multiple of RING][KS][2][64]
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   // column blocks in turn: the tile's low is read while it is in a cache
   const uint32_t tile = blockIdx.x / a.col_blocks, col_block = blockIdx.x % a.col_blocks;
-  const Pair p = seg_pair<16 * TB>(a.g, tile, lane);
-  if (p.hi <= p.lo) return;
+  const Pair p = seg_pair(a.g, RING == 1 ? 16 : a.bm, tile, lane);
+  if (p.hi <= p.lo || (p.adapter < 0 && a.y == a.out)) return;  // (rows without an adapter keep y)
   const int c = lane & 15, g4 = lane >> 4, kg = 8 * g4;
   const int64_t f0 = ((int64_t)col_block * W + wv) * 128, f = f0 + 8 * c;  // this lane's 8 columns
-  const uint16_t* const y = (const uint16_t*)a.y;
-  uint16_t* const out = (uint16_t*)a.out;
-  const uint4 none = make_uint4(0, 0, 0, 0);
-  if (p.adapter < 0) {  // rows without an adapter keep y (dx: zero)
-    if (a.y == a.out || f >= a.n) return;
-    for (int64_t r = p.tile0 + g4; r < p.hi; r += 4)
-      if (r >= p.lo) {
-        uint4 v = none;
-        if (y) v = *(const uint4*)(y + r * a.ys + f);
-        *(uint4*)(out + r * a.os + f) = v;
+  const int rows = (int)(p.hi - p.lo), nb = (rows + 15) / 16;
+  constexpr int kPast = INT32_MAX - 15;  // bytes of a resource, and an offset outside it
+  const uint32_t yo = f < a.n ? 2 * ((uint32_t)(4 * g4) * (uint32_t)a.ys + (uint32_t)f) : kPast;
+  const uint32_t oo = f < a.n ? 2 * ((uint32_t)(4 * g4) * (uint32_t)a.os + (uint32_t)f) : kPast;
+  // rows 16 b + 4 g4 .. + 3 of the pair
+  auto fetch = [&](int b, u32x4(&v)[4]) {
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)((const uint16_t*)a.y + (p.lo + 16 * b) * a.ys), 0,
+                                                      a.y ? kPast : 0, 0x00027000);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = __builtin_amdgcn_raw_buffer_load_b128(
+          rs, 16 * b + 4 * g4 + i < rows ? min(yo + 2 * (uint32_t)(i * a.ys), (uint32_t)kPast) : kPast, 0, 0);
+  };
+  auto store = [&](int b, int i, const uint4& v) {
+    const auto rs =
+        __builtin_amdgcn_make_buffer_rsrc((uint16_t*)a.out + (p.lo + 16 * b) * a.os, 0, kPast, 0x00027000);
+    __builtin_amdgcn_raw_buffer_store_b128(
+        u32x4{v.x, v.y, v.z, v.w}, rs,
+        16 * b + 4 * g4 + i < rows ? min(oo + 2 * (uint32_t)(i * a.os), (uint32_t)kPast) : kPast, 0, 2 /* nt */);
+  };
+  u32x4 yv[RING][4];
+#pragma unroll
+  for (int u = 0; u < RING; ++u) fetch(u, yv[u]);
+  if (p.adapter < 0) {  // (dx: zero)
+    for (int b = 0; b < nb; b += RING)
+#pragma unroll
+      for (int u = 0; u < RING; ++u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) store(b + u, i, make_uint4(yv[u][i][0], yv[u][i][1], yv[u][i][2], yv[u][i][3]));
+        fetch(b + u + RING, yv[u]);
       }
     return;
   }
-  // All of the wave's loads go out at once: y (rows 16 t + 4 g4 .. + 3), the
-  // weights' eight columns, and its share of low. (With y read 16 rows at a
-  // time, a workgroup's chain of loads took twice as long as the bytes need.)
-  uint4 yv[TB][4];
-  if (y) {
-#pragma unroll
-    for (int t = 0; t < TB; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t r = min(max(p.tile0 + 16 * t + 4 * g4 + i, p.lo), p.hi - 1);
-        yv[t][i] = *(const uint4*)(y + r * a.ys + min(f, a.n - 8));
-      }
-  }
+  const uint4 none = make_uint4(0, 0, 0, 0);
   uint4 w[8][KS];
   {
     const uint16_t* wa = (const uint16_t*)a.w + (int64_t)p.adapter * a.n * a.rank;
@@ -304,26 +316,28 @@ __global__ __launch_bounds__(64 * W) void k_lora_expand(ExpandArgs a) {
       for (int s = 0; s < KS; ++s)
         w[j][s] = *(const uint4*)(wa + min(f + j, a.n - 1) * a.rank + min(32 * s + kg, a.rank - 8));
   }
-  // wave w takes fragments w, w + 4, ... of the tile's TB x KS
-  for (int u = wv; u < TB * KS; u += W) {
-    const int t = u / KS, s = u % KS;
-    const int64_t row = p.tile0 + 16 * t + c, rc = min(max(row, p.lo), p.hi - 1);
+  // wave w makes fragments w, w + W, ... of the pair's nb x KS
+  for (int u = wv; u < nb * KS; u += W) {
+    const int s = u % KS;
+    const int64_t row = p.lo + 16 * (u / KS) + c, rc = min(row, p.hi - 1);
     float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (32 * s + kg < a.rank) {
       const int64_t step = a.g.rows * a.rank;
       const float* l = a.low + rc * a.rank + 32 * s + kg;
-      auto add = [&](const float4& x, const float4& y) {
-        f[0] += x.x, f[1] += x.y, f[2] += x.z, f[3] += x.w, f[4] += y.x, f[5] += y.y, f[6] += y.z, f[7] += y.w;
-      };
-      int q = 0;
-      for (; q + 4 <= a.parts; q += 4) {
+      for (int q = 0; q < a.parts; q += 4) {  // four parts' loads in flight
         float4 x[4], y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = *(const float4*)(l + (q + e) * step), y[e] = *(const float4*)(l + (q + e) * step + 4);
+        for (int e = 0; e < 4; ++e) {
+          const float* m = l + min(q + e, a.parts - 1) * step;
+          x[e] = *(const float4*)m, y[e] = *(const float4*)(m + 4);
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) add(x[e], y[e]);
+        for (int e = 0; e < 4; ++e) {
+          if (q + e >= a.parts) break;
+          f[0] += x[e].x, f[1] += x[e].y, f[2] += x[e].z, f[3] += x[e].w;
+          f[4] += y[e].x, f[5] += y[e].y, f[6] += y[e].z, f[7] += y[e].w;
+        }
       }
-      for (; q < a.parts; ++q) add(*(const float4*)(l + q * step), *(const float4*)(l + q * step + 4));
       if (a.low_sum && row == rc && col_block == 0) {
         float* o = a.low_sum + row * a.rank + 32 * s + kg;
         *(float4*)o = make_float4(f[0], f[1], f[2], f[3]);
@@ -332,9 +346,12 @@ __global__ __launch_bounds__(64 * W) void k_lora_expand(ExpandArgs a) {
     }
     uint4 hi, lo;
     split8x<XDT>(f, hi, lo);
-    lows[t][s][0][lane] = hi;
-    lows[t][s][1][lane] = lo;
+    lows[2 * u * 64 + lane] = hi;
+    lows[(2 * u + 1) * 64 + lane] = lo;
   }
+  // Every load so far has ended here, seen by the compiler too: its waits in the
+  // loop would otherwise be for the weights as well, and so for every load.
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
   __syncthreads();
   if (f0 >= a.n) return;  // (no barrier follows)
   if (a.rank < 32 * KS) {  // what is read past the rank counts as 0, whatever it holds
@@ -344,10 +361,7 @@ __global__ __launch_bounds__(64 * W) void k_lora_expand(ExpandArgs a) {
       for (int s = 0; s < KS; ++s)
         if (32 * s + kg >= a.rank) w[j][s] = none;
   }
-#pragma unroll
-  for (int t = 0; t < TB; ++t) {
-    const int64_t r0 = p.tile0 + 16 * t;
-    if (r0 >= p.hi || r0 + 16 <= p.lo) continue;
+  auto block = [&](int b, u32x4(&v)[4]) {
     f32x4 acc[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -355,25 +369,28 @@ __global__ __launch_bounds__(64 * W) void k_lora_expand(ExpandArgs a) {
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int h = 1; h >= 0; --h) {
-        const uint4 l = lows[t][s][h][lane];
+        const uint4 l = lows[(2 * (b * KS + s) + h) * 64 + lane];
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j] = mfma16<XDT>(l, w[j][s], acc[j]);
       }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float o[8];
-      if (y) {
-        unpack8x<XDT>(yv[t][i], o);
+      asm volatile("" : "+v"(v[i]));  // unpacked here, not ahead of the other blocks' loads
+      unpack8x<XDT>(make_uint4(v[i][0], v[i][1], v[i][2], v[i][3]), o);  // (0 where there is no y)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] += acc[j][i];
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = acc[j][i];
-      }
-      const int64_t r = r0 + 4 * g4 + i;
-      if (r >= p.lo && r < p.hi && f < a.n) st_nt16(out + r * a.os + f, pack8x<XDT>(o));
+      for (int j = 0; j < 8; ++j) o[j] += acc[j][i];
+      store(b, i, pack8x<XDT>(o));
     }
-  }
+  };
+  // (a round's blocks past the last have nothing loaded or stored; an exit
+  // between blocks would make the waits of all of them those of the first)
+  for (int b = 0; b < nb; b += RING)
+#pragma unroll
+    for (int u = 0; u < RING; ++u) {
+      block(b + u, yv[u]);
+      if constexpr (RING > 1) fetch(b + u + RING, yv[u]);
+    }
 }
 
 // -------------------------------------------------------- 16-bit transpose
@@ -617,14 +634,28 @@ static void shrink(const ShrinkArgs& a, int parts, hipStream_t s) {
     shrink_launch<XDT, 8>(a, parts, s);
 }
 
-template <int XDT, int KS, int TB, int W>
+// Rows of an expand workgroup where segments are long: the number whose rounds
+// of the CUs cost least, a workgroup's start counted as 24 rows.
+static int expand_rows(int64_t rows, int64_t segments, int64_t col_blocks, int most) {
+  int best = 64;
+  double least = 1e30;
+  for (int bm = 64; bm <= most; bm += 16) {
+    const int64_t wgs = ((rows + bm - 1) / bm + segments - 1) * col_blocks;
+    const double cost = (double)((wgs + cu_count() - 1) / cu_count()) * (bm + 24);
+    if (cost < least) least = cost, best = bm;
+  }
+  return best;
+}
+
+template <int XDT, int KS, int RING, int W>
 static void expand_launch(ExpandArgs a, hipStream_t s) {
   a.col_blocks = (uint32_t)((a.n + 128 * W - 1) / (128 * W));
-  const dim3 grid((unsigned)(seg_pairs(a.g.rows, a.g.count, 16 * TB) * a.col_blocks));
-  k_lora_expand<XDT, KS, TB, W><<<grid, dim3(64 * W), 0, s>>>(a);
+  a.bm = RING == 1 ? 16 : RING == 2 && a.g.rows / a.g.count < 48 ? 32 : expand_rows(a.g.rows, a.g.count, a.col_blocks, 512 / KS);
+  const dim3 grid((unsigned)(seg_pairs(a.g.rows, a.g.count, a.bm) * a.col_blocks));
+  k_lora_expand<XDT, KS, RING, W><<<grid, dim3(64 * W), (a.bm / 16 + RING - 1) / RING * RING * KS * 2048, s>>>(a);
 }
 template <int XDT, int KS>
-static void expand_rows(const ExpandArgs& a, hipStream_t s) {
+static void expand_tiles(const ExpandArgs& a, hipStream_t s) {
   constexpr int most = KS >= 4 ? 2 : 4;
   const int tb = row_blocks(a.g.rows, a.g.count, most);
   if (tb == 4)
@@ -637,11 +668,11 @@ static void expand_rows(const ExpandArgs& a, hipStream_t s) {
 template <int XDT>
 static void expand(const ExpandArgs& a, hipStream_t s) {
   if (a.rank <= 32)
-    expand_rows<XDT, 1>(a, s);
+    expand_tiles<XDT, 1>(a, s);
   else if (a.rank <= 64)
-    expand_rows<XDT, 2>(a, s);
+    expand_tiles<XDT, 2>(a, s);
   else
-    expand_rows<XDT, 4>(a, s);
+    expand_tiles<XDT, 4>(a, s);
 }
 
 static int wgrad_rank_blocks(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : 4; }
@@ -683,6 +714,8 @@ static int lora_shape(int x_dtype, int64_t rows, int64_t k, int64_t n, int64_t r
   return OGA_OK;
 }
 static bool rows_ok(const void* p, int64_t stride) { return p && aligned(p, 16) && stride % 8 == 0; }
+// k_lora_expand's offsets inside 16 rows are 32-bit.
+static bool near_rows(int64_t stride) { return stride >= 0 && stride < (1 << 26); }
 
 static int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
@@ -725,13 +758,15 @@ extern "C" int oga_lora_add(int x_dtype, const void* y, int64_t y_stride, const 
   if (!rows_ok(y, y_stride) || !rows_ok(x, x_stride) || !rows_ok(out, out_stride) || !rows_ok(a, k) ||
       !rows_ok(b, rank) || !aligned(low, 16))
     return fail("operand alignment");
+  if (!near_rows(y_stride) || !near_rows(out_stride))
+    return unsupported("row strides %lld, %lld", (long long)y_stride, (long long)out_stride);
   const int64_t need = oga_lora_add_workspace_bytes(rows, k, rank, segments);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
     return fail("workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   const Segments g = {segment_starts, segment_adapters, (int)segments, (int)adapters, rows};
   const int parts = shrink_parts(rows, segments, k, rank);
   const ShrinkArgs sa = {g, x, x_stride, a, scale, (float*)workspace, k, (int)rank};
-  const ExpandArgs ea = {g, (const float*)workspace, low, b, y, out, y_stride, out_stride, n, (int)rank, parts, 0};
+  const ExpandArgs ea = {g, (const float*)workspace, low, b, y, out, y_stride, out_stride, n, (int)rank, parts, 0, 0};
   const hipStream_t s = (hipStream_t)stream;
   if (x_dtype == OGA_DT_F16) {
     shrink<OGA_DT_F16>(sa, parts, s);
@@ -758,6 +793,7 @@ extern "C" int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, cons
   if (!rows_ok(dy, dy_stride) || !rows_ok(x, x_stride) || !rows_ok(dx, dx_stride) || !rows_ok(a, k) ||
       !rows_ok(b, rank) || !rows_ok(low, 8) || !rows_ok(da, 8) || !rows_ok(db, 8))
     return fail("operand alignment");
+  if (!near_rows(dx_stride)) return unsupported("row stride %lld", (long long)dx_stride);
   const LoraBwdSpace w = lora_bwd_space(rows, k, n, rank, adapters, segments);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < w.total)
     return fail("workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)w.total);
@@ -779,7 +815,7 @@ extern "C" int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, cons
   const Segments g = {segment_starts, segment_adapters, (int)segments, (int)adapters, rows};
   const ShrinkArgs sa = {g, dy, dy_stride, ws + w.bt, scale, parts, n, (int)rank};
   const ExpandArgs ea = {g, parts, w.parts > 1 ? dlow : nullptr, ws + w.at, nullptr, dx, 0, dx_stride, k, (int)rank,
-                         w.parts, 0};
+                         w.parts, 0, 0};
   WgradArgs wa = {};
   wa.g = g, wa.rank = (int)rank, wa.splits = w.splits;
   wa.side[0] = {x, x_stride, dlow, k, (float*)(ws + w.pa), (int)((k + 511) / 512)};
