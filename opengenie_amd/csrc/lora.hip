@@ -12,7 +12,7 @@
 //  * k_lora_expand: the [rows, N] (or [rows, K]) result from low, added to y;
 //    it adds the parts of low up as it reads them, in order.
 //  * k_lora_wgrad: dA and dB, one workgroup per adapter, 512 columns and part
-//    of the adapter's rows; k_lora_join adds the parts in order.
+//    of the adapter's rows; k_lora_join adds the parts, if any, in order.
 // The sums low and dlow stay float32 in memory and enter the matrix products
 // as two 16-bit halves (v = hi + lo), so only results are rounded.
 //
@@ -129,7 +129,7 @@ constexpr int kShrinkWaves = 4;
 // chunks of 64 (a 128-byte line of each row), the waves in turn. The fragments
 // come straight from memory; two chunks of loads are in flight.
 template <int XDT, int RB, int TB>
-__global__ __launch_bounds__(64 * kShrinkWaves) void k_lora_shrink(ShrinkArgs a) {
+__global__ __launch_bounds__(64 * kShrinkWaves, 2) void k_lora_shrink(ShrinkArgs a) {
   __shared__ f32x4 red[kShrinkWaves][TB * RB][64];
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -400,27 +400,41 @@ struct TransposeArgs {
   uint16_t* dst[2];
   int64_t rows[2], cols[2];
   int64_t blocks0;     // workgroups of the first
-  int64_t tiles[2];    // 32 x 32 tiles per adapter
+  int64_t tiles[2];    // 64 x 64 tiles per adapter
   int64_t col_tiles[2];
 };
+// 16 bytes a lane in and out (rows and cols are multiples of 8); the 66-element
+// rows put the eight rows of a lane's column piece into eight banks.
 __global__ __launch_bounds__(256) void k_lora_transpose(TransposeArgs a) {
-  __shared__ uint16_t tile[32][33];
+  __shared__ uint32_t tile[64][33];
   const int i = (int64_t)blockIdx.x >= a.blocks0;
   const int64_t u = (int64_t)blockIdx.x - (i ? a.blocks0 : 0);
   const int64_t rows = i ? a.rows[1] : a.rows[0], cols = i ? a.cols[1] : a.cols[0];
   const int64_t tiles = i ? a.tiles[1] : a.tiles[0], ct = i ? a.col_tiles[1] : a.col_tiles[0];
   const int64_t l = u / tiles, t = u - l * tiles;
-  const int64_t r0 = t / ct * 32, c0 = t % ct * 32;
+  const int64_t r0 = t / ct * 64, c0 = t % ct * 64;
   const uint16_t* src = (i ? a.src[1] : a.src[0]) + l * rows * cols;
   uint16_t* dst = (i ? a.dst[1] : a.dst[0]) + l * rows * cols;
-  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int x = threadIdx.x & 7, y = threadIdx.x >> 3;
 #pragma unroll
-  for (int j = 0; j < 32; j += 8)
-    if (r0 + y + j < rows && c0 + x < cols) tile[y + j][x] = src[(r0 + y + j) * cols + c0 + x];
+  for (int j = 0; j < 64; j += 32)
+    if (r0 + y + j < rows && c0 + 8 * x < cols) {
+      const uint4 v = *(const uint4*)(src + (r0 + y + j) * cols + c0 + 8 * x);
+      uint32_t* o = &tile[y + j][4 * x];
+      o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
+    }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < 32; j += 8)
-    if (c0 + y + j < cols && r0 + x < rows) dst[(c0 + y + j) * rows + r0 + x] = tile[x][y + j];
+  for (int j = 0; j < 64; j += 32)
+    if (c0 + y + j < cols && r0 + 8 * x < rows) {
+      uint32_t v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = tile[8 * x + e][(y + j) >> 1];
+      const uint32_t sel = y & 1 ? 0x07060302u : 0x05040100u;  // (j is even)
+      *(uint4*)(dst + (c0 + y + j) * rows + r0 + 8 * x) =
+          make_uint4(__builtin_amdgcn_perm(v[1], v[0], sel), __builtin_amdgcn_perm(v[3], v[2], sel),
+                     __builtin_amdgcn_perm(v[5], v[4], sel), __builtin_amdgcn_perm(v[7], v[6], sel));
+    }
 }
 
 // ------------------------------------------------------- weight gradients
@@ -430,6 +444,7 @@ struct WgradSide {
   const float* u;    // [rows, rank]: dlow for dA, low for dB
   int64_t c;
   float* part;       // [adapters][splits][rank][c]
+  uint16_t* out;     // where the rows are not split
   int col_tiles;     // of 512 columns
 };
 struct WgradArgs {
@@ -536,6 +551,27 @@ __global__ __launch_bounds__(256) void k_lora_wgrad(WgradArgs a) {
     }
   }
   if (col >= sd.c) return;
+  if (a.splits == 1) {
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      const int rank = r0 + 16 * r + 4 * (lane >> 4);  // .. + 3 (ranks are multiples of 8)
+      if (rank >= a.rank) continue;
+      if (!second) {  // dA [rank][k]
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float f[8] = {acc[0][r][i], acc[1][r][i], acc[2][r][i], acc[3][r][i],
+                              acc[4][r][i], acc[5][r][i], acc[6][r][i], acc[7][r][i]};
+          *(uint4*)(sd.out + ((int64_t)adapter * a.rank + rank + i) * sd.c + col) = pack8x<XDT>(f);
+        }
+      } else {  // dB [n][rank]
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *(uint2*)(sd.out + ((int64_t)adapter * sd.c + col + j) * a.rank + rank) =
+              make_uint2(pack2x<XDT>(acc[j][r][0], acc[j][r][1]), pack2x<XDT>(acc[j][r][2], acc[j][r][3]));
+      }
+    }
+    return;
+  }
   float* part = sd.part + ((int64_t)adapter * a.splits + split) * a.rank * sd.c;
 #pragma unroll
   for (int r = 0; r < RB; ++r)
@@ -594,12 +630,12 @@ static int row_blocks(int64_t rows, int64_t segments, int most) {
 // (Rank 128 holds its weights' fragments for 32 rows at most.)
 static int shrink_tiles(int64_t rank) { return rank > 64 ? 2 : 4; }
 
-// Parts of the long axis: with two (64-row tiles) or three workgroups a CU at
+// Parts of the long axis: with two (64-row tiles, rank 128) or three workgroups a CU at
 // a time, the number whose rounds times a part's length is least (each wave
 // with two chunks or more).
 static int shrink_parts(int64_t rows, int64_t segments, int64_t k, int64_t rank) {
   const int tb = row_blocks(rows, segments, shrink_tiles(rank));
-  const int64_t pairs = seg_pairs(rows, segments, 16 * tb), slots = (tb == 4 ? 2 : 3) * (int64_t)cu_count();
+  const int64_t pairs = seg_pairs(rows, segments, 16 * tb), slots = (tb == 4 || rank > 64 ? 2 : 3) * (int64_t)cu_count();
   const int64_t most = min((k + 63) / 64 / (2 * kShrinkWaves), (int64_t)8);
   int best = 1;
   double least = 1e30;
@@ -637,9 +673,9 @@ static void shrink(const ShrinkArgs& a, int parts, hipStream_t s) {
 // Rows of an expand workgroup where segments are long: the number whose rounds
 // of the CUs cost least, a workgroup's start counted as 24 rows.
 static int expand_rows(int64_t rows, int64_t segments, int64_t col_blocks, int most) {
-  int best = 64;
+  int best = 16;
   double least = 1e30;
-  for (int bm = 64; bm <= most; bm += 16) {
+  for (int bm = 16; bm <= most; bm += 16) {
     const int64_t wgs = ((rows + bm - 1) / bm + segments - 1) * col_blocks;
     const double cost = (double)((wgs + cu_count() - 1) / cu_count()) * (bm + 24);
     if (cost < least) least = cost, best = bm;
@@ -736,6 +772,7 @@ static LoraBwdSpace lora_bwd_space(int64_t rows, int64_t k, int64_t n, int64_t r
   w.pa = w.bt + align256(adapters * rank * n * 2);
   w.pb = w.pa + align256(adapters * w.splits * rank * k * 4);
   w.total = w.pb + align256(adapters * w.splits * rank * n * 4);
+  if (w.splits == 1) w.pb = w.total = w.pa;  // (written straight away)
   if (w.parts == 1) w.dlow = 0;
   return w;
 }
@@ -806,8 +843,8 @@ extern "C" int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, cons
   t.src[0] = (const uint16_t*)a, t.dst[0] = (uint16_t*)(ws + w.at), t.rows[0] = rank, t.cols[0] = k;
   t.src[1] = (const uint16_t*)b, t.dst[1] = (uint16_t*)(ws + w.bt), t.rows[1] = n, t.cols[1] = rank;
   for (int i = 0; i < 2; ++i) {
-    t.col_tiles[i] = (t.cols[i] + 31) / 32;
-    t.tiles[i] = (t.rows[i] + 31) / 32 * t.col_tiles[i];
+    t.col_tiles[i] = (t.cols[i] + 63) / 64;
+    t.tiles[i] = (t.rows[i] + 63) / 64 * t.col_tiles[i];
   }
   t.blocks0 = adapters * t.tiles[0];
   k_lora_transpose<<<dim3((unsigned)(adapters * (t.tiles[0] + t.tiles[1]))), dim3(256), 0, s>>>(t);
@@ -818,8 +855,8 @@ extern "C" int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, cons
                          w.parts, 0, 0};
   WgradArgs wa = {};
   wa.g = g, wa.rank = (int)rank, wa.splits = w.splits;
-  wa.side[0] = {x, x_stride, dlow, k, (float*)(ws + w.pa), (int)((k + 511) / 512)};
-  wa.side[1] = {dy, dy_stride, low, n, (float*)(ws + w.pb), (int)((n + 511) / 512)};
+  wa.side[0] = {x, x_stride, dlow, k, (float*)(ws + w.pa), (uint16_t*)da, (int)((k + 511) / 512)};
+  wa.side[1] = {dy, dy_stride, low, n, (float*)(ws + w.pb), (uint16_t*)db, (int)((n + 511) / 512)};
   JoinArgs j = {};
   j.part[0] = wa.side[0].part, j.part[1] = wa.side[1].part;
   j.out[0] = (uint16_t*)da, j.out[1] = (uint16_t*)db;
@@ -831,12 +868,12 @@ extern "C" int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, cons
     shrink<OGA_DT_F16>(sa, w.parts, s);
     expand<OGA_DT_F16>(ea, s);
     wgrad<OGA_DT_F16>(wa, s);
-    k_lora_join<OGA_DT_F16><<<jgrid, dim3(256), 0, s>>>(j);
+    if (w.splits > 1) k_lora_join<OGA_DT_F16><<<jgrid, dim3(256), 0, s>>>(j);
   } else {
     shrink<OGA_DT_BF16>(sa, w.parts, s);
     expand<OGA_DT_BF16>(ea, s);
     wgrad<OGA_DT_BF16>(wa, s);
-    k_lora_join<OGA_DT_BF16><<<jgrid, dim3(256), 0, s>>>(j);
+    if (w.splits > 1) k_lora_join<OGA_DT_BF16><<<jgrid, dim3(256), 0, s>>>(j);
   }
   return launch_status();
 }
