@@ -492,17 +492,30 @@ __global__ __launch_bounds__(256) void k_lora_wgrad(WgradArgs a) {
     Rows8 cur, nxt;
     rows8(cur, lo);  // in flight while the tile's u goes to LDS
     __syncthreads();  // the last tile's reads are done
-    const int n4 = 4 * RB;  // float4 per row
-    for (int i = threadIdx.x; i < kWgradRows * n4; i += 256) {
-      const int row = i / n4, q = i % n4;
-      float4 v = make_float4(0, 0, 0, 0);
-      if (lo + row < hi && r0 + 4 * q < a.rank) v = *(const float4*)(sd.u + (lo + row) * a.rank + r0 + 4 * q);
-      const float f[4] = {v.x, v.y, v.z, v.w};
+    // a lane: four ranks of rows 2 i, 2 i + 1, which are neighbours in LDS
+    constexpr int kQ = 4 * RB, kIt = kWgradRows / 2 * kQ / 256, kAhead = kIt < 2 ? kIt : 2;
+    const int q = threadIdx.x % kQ, row0 = 2 * (int)(threadIdx.x / kQ);
+    const bool in = r0 + 4 * q < a.rank;
+    const float* up = sd.u + (in ? r0 + 4 * q : 0);
+    for (int it = 0; it < kIt && it * (512 / kQ) < 32 * steps; it += kAhead) {
+      float4 v[2 * kAhead];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t h = pack2x<XDT>(f[e], 0.0f) & 0xFFFFu;
-        uh[(4 * q + e) * kWgradPad + row] = (uint16_t)h;
-        ul[(4 * q + e) * kWgradPad + row] = (uint16_t)(pack2x<XDT>(f[e] - x16_bits<XDT>(h), 0.0f) & 0xFFFFu);
+      for (int e = 0; e < 2 * kAhead; ++e)
+        v[e] = *(const float4*)(up + min(lo + row0 + (it + e / 2) * (512 / kQ) + e % 2, hi - 1) * a.rank);
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) {
+        const int row = row0 + (it + e) * (512 / kQ);
+        const bool in0 = in && lo + row < hi, in1 = in && lo + row + 1 < hi;
+        const float4 &x = v[2 * e], &y = v[2 * e + 1];
+        const float f0[4] = {x.x, x.y, x.z, x.w}, f1[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float a0 = in0 ? f0[i] : 0.0f, a1 = in1 ? f1[i] : 0.0f;
+          const uint32_t h = pack2x<XDT>(a0, a1);
+          *(uint32_t*)(uh + (4 * q + i) * kWgradPad + row) = h;
+          *(uint32_t*)(ul + (4 * q + i) * kWgradPad + row) =
+              pack2x<XDT>(a0 - x16_bits<XDT>(h & 0xFFFFu), a1 - x16_bits<XDT>(h >> 16));
+        }
       }
     }
     __syncthreads();
