@@ -104,16 +104,17 @@ def _torch_lse(q, k, v, scale, causal, k_lens):
     return torch.matmul(p, vf).transpose(1, 2).contiguous().to(q.dtype), lse
 
 
-def _torch_backward(dout, q, k, v, out, lse, scale, causal, k_lens):
+def _torch_backward(dout, q, k, v, lse, scale, causal, k_lens):
     qf, kf, vf, hide = _torch_inputs(q, k, v, causal, k_lens)
-    do, o = (t.to(qf.dtype).transpose(1, 2) for t in (dout, out))
+    do = dout.to(qf.dtype).transpose(1, 2)
     s = torch.matmul(qf, kf.transpose(2, 3).contiguous()) * scale
     if hide is not None:
         s = s.masked_fill(hide, -math.inf)
     lse = lse.to(qf.dtype)
     p = torch.exp(s - lse.masked_fill(lse == -math.inf, 0.0)[..., None])
     dv = torch.matmul(p.transpose(2, 3).contiguous(), do)
-    ds = p * (torch.matmul(do, vf.transpose(2, 3).contiguous()) - (do * o).sum(-1, keepdim=True)) * scale
+    dp = torch.matmul(do, vf.transpose(2, 3).contiguous())
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True)) * scale  # (without out, which is rounded)
     dq, dk = torch.matmul(ds, kf), torch.matmul(ds.transpose(2, 3).contiguous(), qf)
     hk = k.shape[2]
     dk, dv = (t.unflatten(1, (hk, q.shape[2] // hk)).sum(2) for t in (dk, dv))
@@ -161,7 +162,7 @@ def flash_attn_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v:
         return tuple(torch.zeros_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     if not _kernel_ok(q, d, scale) or lse.dtype != torch.float32:
         _fallback("flash_attn_backward", q, k, v)
-        return _torch_backward(dout, q, k, v, out, lse, scale, causal, k_lens)
+        return _torch_backward(dout, q, k, v, lse, scale, causal, k_lens)
     q, qs = heads_layout(q, _MOST)
     k, ks = heads_layout(k, _MOST)
     v, vs = heads_layout(v, _MOST)

@@ -574,7 +574,6 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
   // query that saw no key, and the rows behind the last query up to the
   // tile's 64, get lse2 = +inf, so that their P is 0.
   float lse2[2], delta[2];
-  const int64_t nqt = (a.nq + kGT - 1) / kGT;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int64_t qi = min(q0 + 16 * i + c16, a.nq - 1);
@@ -600,6 +599,53 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
     const float l = a.lse[bh * a.nq + qi];
     const int64_t row = q0 + 16 * i + c16;
     lse2[i] = l == -INFINITY || row >= a.nq ? INFINITY : l * kLog2e;
+  }
+  // out is rounded, and with it Delta, by up to 2^-9 |dO| |out|. Over many keys
+  // |out| is small beside the values and that is lost in dS's own rounding; a
+  // row of few keys sums P (dP - Delta) over them, which is 0 for the exact
+  // Delta, first (9 x 9 causal: dq off by 0.30 % without, by 0.24 % with it).
+  // (Direct loads: these blocks have a few 16-key pieces in all.)
+  constexpr int kFewSteps = CAUSAL ? W / 2 + 1 : 2;
+  if (nsteps <= kFewSteps && q0 < a.nq) {
+    float num[2] = {0.0f, 0.0f}, den[2] = {0.0f, 0.0f};
+#pragma unroll 2
+    for (int64_t key0 = 0; key0 < kend; key0 += 16) {
+      const int64_t ki = min(key0 + c16, nkb - 1);
+      f32x4 s[2], g[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        g[i] = f32x4{-delta[i], -delta[i], -delta[i], -delta[i]};
+      }
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+        const bf16x8 kf = __builtin_bit_cast(bf16x8, *(const uint4*)(kb + ki * a.k_s[1] + 32 * x + 8 * kg));
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, *(const uint4*)(vb + ki * a.v_s[1] + 32 * x + 8 * kg));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s[i] = mfma16(kf, qf[i][x], s[i]), g[i] = mfma16(vf, gf[i][x], g[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int64_t lim = (CAUSAL ? min(nkb, q0 + 16 * i + c16 + shift + 1) : nkb) - key0 - 4 * kg;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][r], a.scale_log2, -lse2[i]));
+          num[i] += r < lim ? p * g[i][r] : 0.0f;
+          den[i] += r < lim ? p : 0.0f;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      num[i] += __shfl_xor(num[i], 16, 64), den[i] += __shfl_xor(den[i], 16, 64);
+      num[i] += __shfl_xor(num[i], 32, 64), den[i] += __shfl_xor(den[i], 32, 64);
+      if (den[i] > 0.0f) delta[i] += num[i] / den[i];
+    }
+  }
+  const int64_t nqt = (a.nq + kGT - 1) / kGT;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int64_t row = q0 + 16 * i + c16;
     if (kg == 0 && row < nqt * kGT && unit.part <= 0) {
       float* t = a.ld + (bh * nqt + row / kGT) * 128 + row % kGT;
       t[0] = lse2[i];
@@ -1114,8 +1160,13 @@ static double causal_fill(const AttnGradArgs& a) {
 
 // The forms of the three kernels: many steps run 8 waves and three tile pairs
 // in one workgroup per CU (D 128); few, or few rows, 4 waves and two pairs in
-// two, one's loads and stores under the other's products.
-static bool few_steps(int64_t own_rows, int64_t other_rows) { return other_rows <= 16 * kGT || own_rows <= 128; }
+// two, one's loads and stores under the other's products. lse / dq / dkv with
+// joins, 32 heads of 128, us, few against many: 1024 x 1024 27 / 40 / 51 against
+// 35 / 38 / 78, 2048 x 2048 causal 54 / 76 / 122 against 62 / 90 / 134, 2304 x
+// 2304 111 / 143 / 202 against 111 / 149 / 214, 4096 x 4096 286 / 384 / 513
+// against 265 / 370 / 516, 128 x 4096 30 / 29 / 49 against 30 / 29 / 57; two
+// sequences of 2304 x 256 39 / 62 / 73 against 46 / 74 / 65.
+static bool few_steps(int64_t own_rows, int64_t other_rows) { return other_rows <= 32 * kGT || own_rows <= 128; }
 static int grad_waves(int64_t head_dim, bool few) { return head_dim == 64 || few ? 4 : 8; }
 static int64_t grad_slots(int64_t head_dim, bool few, int per_cu64) {
   return (int64_t)cu_count() * (head_dim == 64 ? per_cu64 : few ? 2 : 1);
@@ -1129,8 +1180,7 @@ static GradPlan rows_plan(const AttnGradArgs& a, int64_t d, bool dq) {
   return grad_plan(blocks, (a.nk + kGT - 1) / kGT, grad_slots(d, few, 3), step,
                    min((int64_t)rows, a.nq) * (d + (dq ? 0 : 2)) * 4.0, causal_fill(a));
 }
-// (k_attn_dkv's causal 4-wave form would not fit its registers.)
-static bool few_query_steps(const AttnGradArgs& a) { return !a.causal && few_steps(a.nk, a.nq * a.group); }
+static bool few_query_steps(const AttnGradArgs& a) { return few_steps(a.nk, a.nq * a.group); }
 static GradPlan keys_plan(const AttnGradArgs& a, int64_t d) {
   const bool few = few_query_steps(a);
   const int rows = 32 * grad_waves(d, few);
@@ -1242,9 +1292,9 @@ static GradJoin dkv_launch(AttnGradArgs a, const GradPlan& p, hipStream_t s) {
   a.blocks = (int)((a.nk + 32 * W - 1) / (32 * W));
   a.nfull = p.nfull, a.ksplit = p.ksplit;
   const dim3 grid((unsigned)p.units()), block(64 * W);
-  if (a.causal) {
-    if constexpr (D == 64 || W == 8) k_attn_dkv<D, W, BUFS, true><<<grid, block, 0, s>>>(a);
-  } else
+  if (a.causal)
+    k_attn_dkv<D, W, BUFS, true><<<grid, block, 0, s>>>(a);
+  else
     k_attn_dkv<D, W, BUFS, false><<<grid, block, 0, s>>>(a);
   GradJoin j = {a.part, a.dk, a.dv, {}, {}, p.nfull, a.nk, p.ksplit, a.blocks, 32 * W, a.kv_heads, 0,
                 (p.blocks - p.nfull) * 32 * W * (2 * D / 8)};
