@@ -181,6 +181,17 @@ def test_entry_points_refuse_what_the_kernels_do_not_take():
     assert bwd(None, need) == -1 and bwd(p, need - 1) == -1 and bwd(p + 16, need) == -1
 
 
+@pytest.mark.skipif(not _lib.available(), reason="library not built")
+def test_entry_points_refuse_row_strides_past_32_bit_offsets():
+    """Nothing is launched: every call here fails its argument checks."""
+    lib, p = _lib.load(), 4096
+    for ys, outs in ((1 << 26, 64), (64, 1 << 26), (-64, 64), (64, -64)):
+        assert lib.oga_lora_add(0, p, ys, p, 64, p, p, None, p, p, 1, 1, p, p, outs, 4, 64, 64, 8, p, 1 << 40, None) == -2
+    for dxs in (1 << 26, -64):
+        assert lib.oga_lora_bwd(0, p, 64, p, 64, p, p, p, None, p, p, 1, 1, p, dxs, p, p, 4, 64, 64, 8, p, 1 << 40,
+                                None) == -2
+
+
 # ------------------------------------------------------------------- GPU
 SEGMENTS = [
     ([0, 1], [0]), ([0, 70], [1]), ([3, 3, 20, 64, 65, 67], [0, 1, 5, 2, -1]), ([0, 16, 32, 48, 64, 80], [2, 2, 0, 1, 2]),
@@ -205,6 +216,19 @@ def test_gpu_against_float64(rank, dtype, monkeypatch):
             c["scale"] = None
         run_and_check(c, starts, ids, torch.int64 if i % 3 == 0 else torch.int32)
     assert L.collect_hip_calls() == {"lora_add": len(SEGMENTS), "lora_backward": len(SEGMENTS)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rank", [8, 64, 128])
+def test_gpu_long_segments_against_float64(rank, dtype):
+    """Workgroups that stream several rounds of rows, whole and cut short, with
+    and without an adapter, and columns that end inside a wave's 128."""
+    for rows, k, n, starts, ids in ((6001, 72, 4104, [3, 2900, 5989], [1, 0]), (4999, 2056, 136, [0, 4000, 4500, 4999], [0, 7, 1])):
+        c = case(rows, k, n, rank, 2, dtype, "cuda", seed=rows)
+        want = run_and_check(c, starts, ids)
+        y, rest = c["y"].clone(), (c["a"], c["b"], c["scale"], *segs(starts, ids, "cuda"))
+        assert torch.equal(A.lora_add(y, c["x"], *rest, out=y), want[0])
 
 
 @pytest.mark.gpu
