@@ -12,12 +12,19 @@
 //
 // Three kernels share one loop shape: a wave keeps its own rows in registers
 // and walks 64-row tiles of the other side, which LDS-DMA brings into a ring
-// of three tile pairs, two steps ahead (k_attn_lse: 32 queries a wave over K
-// and V; k_attn_dq: the same for dq; k_attn_dkv: 32 keys a wave over Q and dO
-// of all query heads of the group). No sum crosses a workgroup by atomics:
-// recomputing S and dP in both gradient kernels (7 products where 5 would do)
-// costs less than writing and joining partial dq, and results do not depend on
-// the order of workgroups.
+// of three tile pairs, two steps ahead, or two where steps are few
+// (k_attn_lse: 32 queries a wave over K and V; k_attn_dq: the same for dq;
+// k_attn_dkv: 32 keys a wave over Q and dO of all query heads of the group).
+// No sum crosses a workgroup by atomics: recomputing S and dP in both gradient
+// kernels (7 products where 5 would do) costs less than writing and joining
+// partial dq, and results do not depend on the order of workgroups. Blocks that
+// would leave CUs idle are cut over their steps and joined in a fixed order.
+//
+// What bounds them: at D 128 the MFMAs and the power they draw (9216 x 9216, 32
+// heads: busy 0.56 to 0.60 of the cycles), at D 64, with half the products per
+// score, the exponentials and conversions (VALU 0.58 to 0.70, MFMA 0.41 to 0.50
+// at 4099 x 4099 causal), over 256 keys the rows of Q, dO, out and the results
+// (2 x 2304 rows: MFMA 0.22 to 0.32).
 #include "common.h"
 #include "host.h"
 
@@ -259,6 +266,8 @@ OGA_DEVICE float sum_halves(float v) {
 // W waves of 32 queries. S^T = K Q^T in 32 x 32 blocks (lane l: query l % 32,
 // keys 8g + 4 (l / 32) + r), online softmax in base 2 with the running max
 // moved only when a score passes it by 8 (P stays below 2^8), O^T += V^T P^T.
+// 9216 x 9216, 32 heads of 128: 1215 us, 1145 TFLOP/s of its two products; 4099
+// x 4099 causal, 32 / 8 heads of 64: 98 us.
 template <int D, int W, int BUFS, bool CAUSAL>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void k_attn_lse(
     AttnGradArgs a) {
@@ -525,12 +534,15 @@ __global__ __launch_bounds__(256) void k_attn_lse_join(AttnGradArgs a) {
 }
 
 // --------------------------------------------------------------------- dq
-// 8 waves of 32 queries over tiles of 64 keys. S^T = K Q^T and dP^T = V dO^T
+// W waves of 32 queries over tiles of 64 keys. S^T = K Q^T and dP^T = V dO^T
 // in 16 x 16 blocks (lane l: query l % 16, keys 4 (l / 16) + r), so a lane's
 // lse and Delta are two numbers; dq^T += K^T dS^T with K^T by transposing
 // reads, whose 32 keys' order (4 (l / 16) + r of two 16-key blocks) is that of
-// the blocks' accumulators. 16x16x32 MFMAs draw less power than 32x32x16 at
-// the same rate, and no row maximum is needed here.
+// the blocks' accumulators. 16x16x32 MFMAs reach 2083 TFLOP/s where 32x32x16
+// reach 1585 (registers only, random operands: power), and no row maximum, for
+// which a query should stay in two lanes, is needed here. 9216 x 9216, 32 heads
+// of 128: 1604 us, 1301 TFLOP/s of its three products; 4099 x 4099 causal, 32 /
+// 8 heads of 64: 122 us.
 template <int D, int W, int BUFS, bool CAUSAL>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void k_attn_dq(
     AttnGradArgs a) {
@@ -791,11 +803,13 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
 }
 
 // ------------------------------------------------------------- dk and dv
-// 8 waves of 32 keys (K and V in registers as B operands) over tiles of 64
+// W waves of 32 keys (K and V in registers as B operands) over tiles of 64
 // queries of every query head of the group. S = Q K^T and dP = dO V^T in
 // 16 x 16 blocks (lane l: key l % 16, queries 4 (l / 16) + r), whose lse and
 // Delta come from LDS, four queries a read; dv^T += dO^T P and dk^T += Q^T dS
-// with the transposed tiles by transposing reads.
+// with the transposed tiles by transposing reads. 9216 x 9216, 32 heads of 128:
+// 2242 us, 1241 TFLOP/s of its four products; 4099 x 4099 causal, 32 / 8 heads of
+// 64: 170 us.
 template <int D, int W, int BUFS, bool CAUSAL>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2))) void k_attn_dkv(
     AttnGradArgs a) {
@@ -1066,7 +1080,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
 }
 
 // The gradients of the blocks that ran in parts, added in part order; 8 values
-// a thread. Side 0: dq (rows of D), side 1: dk and dv (rows of 2 D).
+// a thread (2 x 2304 x 256: 75 MB in 12.7 us). Side 0: dq (rows of D), side 1: dk and dv (rows of 2 D).
 struct GradJoin {
   const float* part;
   uint16_t *o, *o2;

@@ -17,7 +17,8 @@
 // 16-bit inputs (4 dwords for 8 elements; its norm factor is the same row's).
 // A wave takes one token's heads (several tokens' where a token has fewer
 // heads than the wave has rows) NV rows a lane at a time, so the token's
-// angles are read once for NV rows.
+// angles are read once for NV rows. 9216 tokens, 32 + 32 heads of 128: 68 us,
+// 4.5 TB/s; 4999 tokens, 64 heads of 64: 18.4 us forward, 28.5 back, 4.4 TB/s.
 #include "common.h"
 #include "host.h"
 
