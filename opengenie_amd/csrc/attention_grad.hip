@@ -1225,8 +1225,9 @@ static int grad_shape(AttnGradArgs& a, int64_t batch, int64_t nq, int64_t nk, in
                 (long long)heads, (long long)kv_heads);
   if (nq > (1 << 30) || nk > (1 << 30) || heads > (1 << 20) || batch > (1 << 20))
     return unsupported("shape (%lld, %lld, %lld, %lld)", (long long)batch, (long long)nq, (long long)nk, (long long)heads);
-  if (batch * heads * ((nq + 31) / 32) > INT32_MAX / 16 || batch * kv_heads * ((nk + 31) / 32) > INT32_MAX / 16)
-    return unsupported("more than 2^31 workgroups");
+  // a grid holds less than 2^32 threads: 256 for 128 rows
+  if (batch * heads * ((nq + 127) / 128) >= 1 << 24 || batch * kv_heads * ((nk + 127) / 128) >= 1 << 24)
+    return unsupported("more than 2^24 blocks of 128 rows");
   if ((nq + kGT - 1) / kGT * (heads / kv_heads) > INT32_MAX / 64) return unsupported("too many queries per key head");
   if (!(scale > 0.0f) || scale > 1e30f) return fail("softmax scale");
   if (!aligned(k_lens, 4)) return fail("k_lens alignment");

@@ -768,6 +768,10 @@ static int lora_shape(int x_dtype, int64_t rows, int64_t k, int64_t n, int64_t r
     return fail("%lld adapters, %lld segments", (long long)adapters, (long long)segments);
   if (rows > (1 << 30) || k > (1 << 22) || n > (1 << 22))
     return unsupported("rows %lld, k %lld, n %lld", (long long)rows, (long long)k, (long long)n);
+  // a grid holds less than 2^32 threads: 256 for 16 rows and 512 columns
+  if (((rows + 15) / 16 + segments + 2) * ((max(k, n) + 511) / 512) >= 1 << 24)
+    return unsupported("%lld rows, %lld segments of %lld, %lld columns", (long long)rows, (long long)segments, (long long)k,
+                       (long long)n);
   if (!starts || !ids || !aligned(starts, 4) || !aligned(ids, 4)) return fail("segments");
   return OGA_OK;
 }

@@ -177,6 +177,7 @@ def test_entry_points_refuse_what_the_kernels_do_not_take():
                {"scale": float("nan")}, {"scale": float("inf")}):
         assert lse(**kw) == -1, kw
     assert lse(nq=1 << 31) == -2 and lse(batch=1 << 20, heads=1 << 20) == -2
+    assert lse(batch=1 << 19, heads=32) == -2 and lse(batch=1 << 19, nq=8, nk=4096) == -2  # grids past 2^32 threads
     need = lib.oga_attention_lse_workspace_bytes(1, 4, 4096, 1, 1, 128, 0)
     assert need > 0  # one block, cut over its keys
     for kw in ({}, {"ws": p, "size": need - 1}, {"ws": p + 16, "size": need}):

@@ -182,6 +182,17 @@ def test_entry_points_refuse_what_the_kernels_do_not_take():
 
 
 @pytest.mark.skipif(not _lib.available(), reason="library not built")
+def test_entry_points_refuse_grids_past_the_hardware_limit():
+    """Nothing is launched: every call here fails its argument checks."""
+    lib, p = _lib.load(), 4096
+    for rows, n, segments in ((1 << 28, 64, 1), (1 << 20, 1 << 17, 1), (4, 1 << 16, 1 << 20)):
+        assert lib.oga_lora_add(0, p, n, p, 64, p, p, None, p, p, segments, 1, p, p, n, rows, 64, n, 8, p, 1 << 60,
+                                None) == -2
+        assert lib.oga_lora_bwd(0, p, n, p, 64, p, p, p, None, p, p, segments, 1, p, 64, p, p, rows, 64, n, 8, p, 1 << 60,
+                                None) == -2
+
+
+@pytest.mark.skipif(not _lib.available(), reason="library not built")
 def test_entry_points_refuse_row_strides_past_32_bit_offsets():
     """Nothing is launched: every call here fails its argument checks."""
     lib, p = _lib.load(), 4096
