@@ -520,7 +520,7 @@ int oga_head_rmsnorm_rope_bwd(int x_dtype, const void* dq_out, const int64_t dqo
 /*
  * Low-rank adapters of many requests beside a shared projection. No
  * counterpart in the reference. y, out [rows, n], x [rows, k] bf16 or fp16
- * with row strides (multiples of 8, y's and out's below 2^26, 16-byte aligned
+ * with row strides (multiples of 8, y's and out's below 2^25, 16-byte aligned
  * bases; out may be y);
  * a [adapters, rank, k], b [adapters, n, rank] contiguous, scale [adapters]
  * float32 or NULL (1); rank a multiple of 8 up to 128, k and n multiples of 8.
@@ -545,7 +545,7 @@ int oga_lora_add(int x_dtype, const void* y, int64_t y_stride, const void* x, in
  * Backward pass of oga_lora_add (y's gradient is dy itself): dx [rows, k] =
  * scale a^T (b^T dy) (0 in rows without an adapter), da and db in a's and b's
  * layouts, summed over each adapter's rows in float32 in a fixed order (0 for
- * an adapter without rows). dx's row stride is below 2^26. Workspace (256-byte
+ * an adapter without rows). Row strides are below 2^25. Workspace (256-byte
  * aligned) of oga_lora_bwd_workspace_bytes(...) bytes on the current device.
  */
 int64_t oga_lora_bwd_workspace_bytes(int64_t rows, int64_t k, int64_t n, int64_t rank, int64_t adapters,

@@ -49,12 +49,12 @@ def heads_layout(t: torch.Tensor, most: int = 1 << 62) -> tuple[torch.Tensor, tu
 
 def rows_layout(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """t (..., C) as rows of C, and the row stride: unit stride along C,
-    16-byte aligned rows, strides below 2^26; a copy where t is laid out
+    16-byte aligned rows, strides below 2^25; a copy where t is laid out
     otherwise."""
     if t.ndim != 2:
         t = t.reshape(-1, t.shape[-1])
     stride, unit = t.stride()
-    if unit != 1 or stride & 7 or stride >= 1 << 26 or t.data_ptr() & 15:
+    if unit != 1 or stride & 7 or stride >= 1 << 25 or t.data_ptr() & 15:
         if t.shape[0] == 1 and (unit == 1 or t.shape[1] == 1) and not t.data_ptr() & 15:
             return t, 0
         t = t.clone(memory_format=torch.contiguous_format)

@@ -62,6 +62,9 @@ OGA_DEVICE void split8x(const float* f, uint4& hi, uint4& lo) {
   lo = pack8x<XDT>(d);
 }
 
+// Bytes of a buffer resource, and an offset outside it.
+constexpr int kPast = INT32_MAX - 15;
+
 struct Segments {
   const int32_t* starts;  // [count + 1]
   const int32_t* ids;     // [count]
@@ -278,7 +281,6 @@ __global__ __launch_bounds__(64 * W) void k_lora_expand(ExpandArgs a) {
   const int c = lane & 15, g4 = lane >> 4, kg = 8 * g4;
   const int64_t f0 = ((int64_t)col_block * W + wv) * 128, f = f0 + 8 * c;  // this lane's 8 columns
   const int rows = (int)(p.hi - p.lo), nb = (rows + 15) / 16;
-  constexpr int kPast = INT32_MAX - 15;  // bytes of a resource, and an offset outside it
   const uint32_t yo = f < a.n ? 2 * ((uint32_t)(4 * g4) * (uint32_t)a.ys + (uint32_t)f) : kPast;
   const uint32_t oo = f < a.n ? 2 * ((uint32_t)(4 * g4) * (uint32_t)a.os + (uint32_t)f) : kPast;
   // rows 16 b + 4 g4 .. + 3 of the pair
@@ -460,7 +462,8 @@ struct WgradArgs {
 constexpr int kWgradRows = 128;  // rows of one pass over LDS
 constexpr int kWgradPad = kWgradRows + 8;
 
-// (4608 rows of x and dy of 4096, rank 32: 26.8 us, 2.8 TB/s.)
+// (4608 rows of x and dy of 4096, rank 32: 23.8 us, 3.2 TB/s; 26.5 with each
+// step's rows waited for by a register copy.)
 // One adapter, 4 x 128 columns, ranks 16 RB z .. , every splits-th 128-row
 // tile of the adapter's segments. A lane loads 8 rows x 8 columns (16 lanes
 // cover 256 bytes of a row) and regroups them by column with one v_perm per
@@ -484,25 +487,28 @@ __global__ __launch_bounds__(256) void k_lora_wgrad(WgradArgs a) {
 #pragma unroll
     for (int r = 0; r < RB; ++r) acc[j][r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   int64_t seen = 0;  // tiles of this adapter so far
-  struct Rows8 {
-    uint4 v[8];
-  };
+  typedef u32x4 Rows8[8];
+  const uint32_t xs2 = 2 * (uint32_t)sd.xs, x0 = (uint32_t)g8 * xs2 + 2 * (uint32_t)colc;
   auto tile = [&](int64_t lo, int64_t hi) {
-    const int steps = (int)((min(hi - lo, (int64_t)kWgradRows) + 31) / 32);
-    auto rows8 = [&](Rows8& x, int64_t first) {
+    const int rows = (int)min(hi - lo, (int64_t)kWgradRows), steps = (rows + 31) / 32;
+    // rows 32 st + g8 .. + 7; 0 past the segment's end, whose rows may hold anything
+    auto rows8 = [&](Rows8& x, int st) {
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)((const uint16_t*)sd.x + (lo + 32 * st) * sd.xs), 0,
+                                                        kPast, 0x00027000);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        x.v[j] = *(const uint4*)((const uint16_t*)sd.x + min(first + g8 + j, hi - 1) * sd.xs + colc);
+        x[j] = __builtin_amdgcn_raw_buffer_load_b128(rs, 32 * st + g8 + j < rows ? x0 + j * xs2 : (uint32_t)kPast, 0, 0);
     };
     Rows8 cur, nxt;
-    rows8(cur, lo);  // in flight while the tile's u goes to LDS
+    rows8(cur, 0);  // in flight while the tile's u goes to LDS
+    rows8(nxt, 1);
     __syncthreads();  // the last tile's reads are done
     // a lane: four ranks of rows 2 i, 2 i + 1, which are neighbours in LDS
     constexpr int kQ = 4 * RB, kIt = kWgradRows / 2 * kQ / 256, kAhead = kIt < 2 ? kIt : 2;
     const int q = threadIdx.x % kQ, row0 = 2 * (int)(threadIdx.x / kQ);
     const bool in = r0 + 4 * q < a.rank;
     const float* up = sd.u + (in ? r0 + 4 * q : 0);
-    for (int it = 0; it < kIt && it * (512 / kQ) < 32 * steps; it += kAhead) {
+    for (int it = 0; it < kIt && it * (512 / kQ) < 64 * ((steps + 1) / 2); it += kAhead) {
       float4 v[2 * kAhead];
 #pragma unroll
       for (int e = 0; e < 2 * kAhead; ++e)
@@ -524,13 +530,7 @@ __global__ __launch_bounds__(256) void k_lora_wgrad(WgradArgs a) {
       }
     }
     __syncthreads();
-    for (int st = 0; st < steps; ++st) {
-      rows8(nxt, lo + 32 * (st + 1));  // (past the end: the last row again)
-      if (lo + 32 * st + 32 > hi) {    // rows of others may hold anything
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (lo + 32 * st + g8 + j >= hi) cur.v[j] = make_uint4(0, 0, 0, 0);
-      }
+    auto mul = [&](const Rows8& x, int st) {
       uint4 fh[RB], fl[RB];
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
@@ -541,18 +541,26 @@ __global__ __launch_bounds__(256) void k_lora_wgrad(WgradArgs a) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
-        auto word = [&](const uint4& v) { return (j >> 1) == 0 ? v.x : (j >> 1) == 1 ? v.y : (j >> 1) == 2 ? v.z : v.w; };
-        const uint4 xf = make_uint4(__builtin_amdgcn_perm(word(cur.v[1]), word(cur.v[0]), sel),
-                                    __builtin_amdgcn_perm(word(cur.v[3]), word(cur.v[2]), sel),
-                                    __builtin_amdgcn_perm(word(cur.v[5]), word(cur.v[4]), sel),
-                                    __builtin_amdgcn_perm(word(cur.v[7]), word(cur.v[6]), sel));
+        const uint4 xf = make_uint4(__builtin_amdgcn_perm(x[1][j >> 1], x[0][j >> 1], sel),
+                                    __builtin_amdgcn_perm(x[3][j >> 1], x[2][j >> 1], sel),
+                                    __builtin_amdgcn_perm(x[5][j >> 1], x[4][j >> 1], sel),
+                                    __builtin_amdgcn_perm(x[7][j >> 1], x[6][j >> 1], sel));
 #pragma unroll
         for (int r = 0; r < RB; ++r) {
           acc[j][r] = mfma16<XDT>(fl[r], xf, acc[j][r]);
           acc[j][r] = mfma16<XDT>(fh[r], xf, acc[j][r]);
         }
       }
-      cur = nxt;
+    };
+    // Two steps at a time (a copy of rows in flight would wait for them), and
+    // none of the second's work before the first's next loads.
+    for (int st = 0; st < steps; st += 2) {
+      mul(cur, st);
+      rows8(cur, st + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      mul(nxt, st + 1);
+      rows8(nxt, st + 3);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   for (int s0 = 0; s0 < a.g.count; s0 += 64) {
@@ -776,8 +784,8 @@ static int lora_shape(int x_dtype, int64_t rows, int64_t k, int64_t n, int64_t r
   return OGA_OK;
 }
 static bool rows_ok(const void* p, int64_t stride) { return p && aligned(p, 16) && stride % 8 == 0; }
-// k_lora_expand's offsets inside 16 rows are 32-bit.
-static bool near_rows(int64_t stride) { return stride >= 0 && stride < (1 << 26); }
+// Offsets inside 16 or 32 rows are 32-bit.
+static bool near_rows(int64_t stride) { return stride >= 0 && stride < (1 << 25); }
 
 static int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
@@ -856,7 +864,8 @@ extern "C" int oga_lora_bwd(int x_dtype, const void* dy, int64_t dy_stride, cons
   if (!rows_ok(dy, dy_stride) || !rows_ok(x, x_stride) || !rows_ok(dx, dx_stride) || !rows_ok(a, k) ||
       !rows_ok(b, rank) || !rows_ok(low, 8) || !rows_ok(da, 8) || !rows_ok(db, 8))
     return fail("operand alignment");
-  if (!near_rows(dx_stride)) return unsupported("row stride %lld", (long long)dx_stride);
+  if (!near_rows(dy_stride) || !near_rows(x_stride) || !near_rows(dx_stride))
+    return unsupported("row strides %lld, %lld, %lld", (long long)dy_stride, (long long)x_stride, (long long)dx_stride);
   const LoraBwdSpace w = lora_bwd_space(rows, k, n, rank, adapters, segments);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < w.total)
     return fail("workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)w.total);

@@ -198,8 +198,8 @@ def test_entry_points_refuse_row_strides_past_32_bit_offsets():
     lib, p = _lib.load(), 4096
     for ys, outs in ((1 << 26, 64), (64, 1 << 26), (-64, 64), (64, -64)):
         assert lib.oga_lora_add(0, p, ys, p, 64, p, p, None, p, p, 1, 1, p, p, outs, 4, 64, 64, 8, p, 1 << 40, None) == -2
-    for dxs in (1 << 26, -64):
-        assert lib.oga_lora_bwd(0, p, 64, p, 64, p, p, p, None, p, p, 1, 1, p, dxs, p, p, 4, 64, 64, 8, p, 1 << 40,
+    for dys, xs, dxs in ((64, 64, 1 << 26), (64, 64, -64), (64, 1 << 26, 64), (1 << 26, 64, 64)):
+        assert lib.oga_lora_bwd(0, p, dys, p, xs, p, p, p, None, p, p, 1, 1, p, dxs, p, p, 4, 64, 64, 8, p, 1 << 40,
                                 None) == -2
 
 
