@@ -31,6 +31,18 @@ def bytes_on(t: torch.Tensor, name: str, *args) -> int:
         return _lib.function(name)(*args)
 
 
+def fresh(t: torch.Tensor) -> torch.Tensor:
+    """An empty contiguous tensor of t's shape, dtype and device (empty_like
+    takes half of empty's time with all of them named)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
+def scratch(t: torch.Tensor, size: int) -> torch.Tensor:
+    """size bytes, an even number, on the device of t, a 16-bit tensor (in its
+    own dtype, which new_empty need not be told)."""
+    return t.new_empty(size >> 1)
+
+
 def heads_layout(t: torch.Tensor, most: int = 1 << 62) -> tuple[torch.Tensor, tuple[int, int, int]]:
     """t [B, N, H, D] as the kernels read it, and its (batch, token, head)
     strides: unit stride along D, 16-byte aligned rows, token and head strides

@@ -23,7 +23,7 @@ import math
 
 import torch
 
-from ._launch import bytes_on, call_on, heads_layout
+from ._launch import bytes_on, call_on, fresh, heads_layout, scratch
 from .ltx_ops import _fallback, _hip
 
 __all__ = ["flash_attn_lse", "flash_attn_backward", "attention_with_grad"]
@@ -138,11 +138,10 @@ def flash_attn_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_sc
     k, ks = heads_layout(k, _MOST)
     v, vs = heads_layout(v, _MOST)
     lens = _lens32(k_lens, nk)
-    dev = q.device
-    out = torch.empty((b, nq, h, d), device=dev, dtype=torch.bfloat16)
-    lse = torch.empty((b, h, nq), device=dev, dtype=torch.float32)
+    out = fresh(q)
+    lse = q.new_empty((b, h, nq), dtype=torch.float32)
     size = bytes_on(q, "oga_attention_lse_workspace_bytes", b, nq, nk, h, hk, d, bool(causal))
-    ws = torch.empty((size,), device=dev, dtype=torch.uint8) if size else None
+    ws = scratch(q, size) if size else None
     _hip("flash_attn_lse")
     call_on(q, "oga_attention_lse", q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(),
             (nq * h * d, h * d, d), lse.data_ptr(), b, nq, nk, h, hk, d, scale, bool(causal),
@@ -171,13 +170,10 @@ def flash_attn_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v:
     if not lse.is_contiguous():
         lse = lse.contiguous()
     lens = _lens32(k_lens, nk)
-    dev = q.device
-    dq = torch.empty((b, nq, h, d), device=dev, dtype=torch.bfloat16)
-    dk = torch.empty((b, nk, hk, d), device=dev, dtype=torch.bfloat16)
-    dv = torch.empty_like(dk)
+    dq, dk, dv = fresh(q), fresh(k), fresh(v)
     dqs, dks = (nq * h * d, h * d, d), (nk * hk * d, hk * d, d)
     size = bytes_on(q, "oga_attention_bwd_workspace_bytes", b, nq, nk, h, hk, d, bool(causal))
-    ws = torch.empty((size,), device=dev, dtype=torch.uint8)
+    ws = scratch(q, size)
     _hip("flash_attn_backward")
     call_on(q, "oga_attention_bwd", dout.data_ptr(), ds, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
             out.data_ptr(), os, lse.data_ptr(), dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(), dks, b, nq, nk,

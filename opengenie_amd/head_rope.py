@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import torch
 
-from ._launch import bytes_on, call_on, heads_layout, vector32
+from ._launch import bytes_on, call_on, fresh, heads_layout, scratch, vector32
 from .ltx_ops import _any_dt, _fallback, _hip, _xdt
 
 __all__ = ["qk_head_rmsnorm_rope", "qk_head_rmsnorm_rope_backward", "qk_head_rmsnorm_rope_with_grad", "apply_rope"]
@@ -140,12 +140,12 @@ def _torch_norm_turn_grad(dy, x, w, eps, cos, sin, layout):
 def _forward(q, k, q_weight, k_weight, eps, cos, sin, layout, positions, norm, inverse):
     b, n, h, d = q.shape
     q, qs = heads_layout(q)
-    q_out = torch.empty((b, n, h, d), device=q.device, dtype=q.dtype)
+    q_out = fresh(q)
     hk, k_out, kp, kop, ks, kos = 0, None, None, None, (0, 0, 0), (0, 0, 0)
     if k is not None:
         hk = k.shape[2]
         k, ks = heads_layout(k)
-        k_out = torch.empty((b, n, hk, d), device=q.device, dtype=q.dtype)
+        k_out = fresh(k)
         kos = (n * hk * d, hk * d, d)
         kp, kop = k.data_ptr(), k_out.data_ptr()
     qw, kw, wdt = _weights(q_weight, k_weight)
@@ -202,8 +202,7 @@ def qk_head_rmsnorm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q:
     k, ks = heads_layout(k)
     dq_out, dqos = heads_layout(dq_out)
     dk_out, dkos = heads_layout(dk_out)
-    dq = torch.empty((b, n, h, d), device=q.device, dtype=q.dtype)
-    dk = torch.empty((b, n, hk, d), device=q.device, dtype=q.dtype)
+    dq, dk = fresh(q), fresh(k)
     qw, kw, wdt = _weights(q_weight, k_weight)
     dqw, dkw = (None if w is None else torch.empty((d,), device=q.device, dtype=wdt) for w in (qw, kw))
     cos, sin, row = _tables(cos, sin)
@@ -211,7 +210,7 @@ def qk_head_rmsnorm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q:
     ws, size = None, 0
     if qw is not None or kw is not None:
         size = bytes_on(q, "oga_head_rmsnorm_rope_bwd_workspace_bytes", d)
-        ws = torch.empty((size,), device=q.device, dtype=torch.uint8)
+        ws = scratch(q, size)
     call_on(q, "oga_head_rmsnorm_rope_bwd", _xdt(q), dq_out.data_ptr(), dqos, dk_out.data_ptr(), dkos, q.data_ptr(),
             qs, k.data_ptr(), ks, _ptr(qw), _ptr(kw), 0 if wdt == torch.bfloat16 else 1, cos.data_ptr(),
             sin.data_ptr(), _any_dt(cos), row, cos.shape[0], pos, pos64, pos_strides, dq.data_ptr(),

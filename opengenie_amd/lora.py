@@ -27,7 +27,7 @@ from dataclasses import dataclass
 
 import torch
 
-from ._launch import bytes_on, call_on, rows_layout
+from ._launch import bytes_on, call_on, fresh, rows_layout, scratch
 from .ltx_ops import _fallback, _hip, _xdt, fp8_linear_forward
 
 _INDEX = (torch.int32, torch.int64)
@@ -134,15 +134,15 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
         r = r if out is None else out.copy_(r)
         return (r, low.reshape(rows, -1, rank).sum(1)) if save_low else r
     if out is None:
-        out = torch.empty(shape, device=y.device, dtype=y.dtype)
+        out = fresh(y)
     x2, xs = rows_layout(x)
     y2, ys = rows_layout(y)
-    low = torch.empty((rows, rank), device=x.device, dtype=torch.float32) if save_low else None
+    low = x.new_empty((rows, rank), dtype=torch.float32) if save_low else None
     a, b = _packed(a), _packed(b)
     scale = scale if scale is None or scale.is_contiguous() else scale.contiguous()
     starts, ids = _i32(segment_starts, rows), _i32(segment_adapters, adapters)
     size = bytes_on(x, "oga_lora_add_workspace_bytes", rows, k, rank, segments)
-    ws = torch.empty((size,), device=x.device, dtype=torch.uint8)
+    ws = scratch(x, size)
     _hip("lora_add")
     call_on(x, "oga_lora_add", _xdt(x), y2.data_ptr(), ys, x2.data_ptr(), xs, a.data_ptr(), b.data_ptr(),
             None if scale is None else scale.data_ptr(), starts.data_ptr(), ids.data_ptr(), segments, adapters,
@@ -175,7 +175,7 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, low: torch.Tensor, a: torch
         da = torch.matmul(dlow.t(), xf).reshape(a.shape).to(a.dtype)
         db = torch.matmul(mine.t(), df).reshape(a.shape[0], rank, n).transpose(1, 2).contiguous().to(b.dtype)
         return dx, da, db
-    dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    dx = fresh(x)
     x2, xs = rows_layout(x)
     dy2, dys = rows_layout(dy)
     low, a, b = _packed(low), _packed(a), _packed(b)
@@ -183,7 +183,7 @@ def lora_backward(dy: torch.Tensor, x: torch.Tensor, low: torch.Tensor, a: torch
     starts, ids = _i32(segment_starts, rows), _i32(segment_adapters, adapters)
     da, db = torch.empty_like(a), torch.empty_like(b)
     size = bytes_on(x, "oga_lora_bwd_workspace_bytes", rows, k, n, rank, adapters, segments)
-    ws = torch.empty((size,), device=x.device, dtype=torch.uint8)
+    ws = scratch(x, size)
     _hip("lora_backward")
     call_on(x, "oga_lora_bwd", _xdt(x), dy2.data_ptr(), dys, x2.data_ptr(), xs, low.data_ptr(), a.data_ptr(),
             b.data_ptr(), None if scale is None else scale.data_ptr(), starts.data_ptr(), ids.data_ptr(),
