@@ -453,7 +453,8 @@ int64_t oga_rows_per_wave(int kind, int64_t batch, int64_t tokens, int64_t cols)
  * j <= i + k_lens[b] - Nq (the last query sees every valid key). A query that
  * sees no key has o = 0, lse = -inf and no gradient. Scores and sums are
  * float32, P and dS round to bf16 for the second products, results once.
- * sum(dout o) is corrected, where rows see few keys, for o's rounding.
+ * sum(dout o) is corrected, where rows see few keys (48; causal, the first 128),
+ * for o's rounding.
  * Nothing is summed by atomics: the same call gives the same bits.
  * Workspaces (256-byte aligned) of the queries' bytes on the current device;
  * the forward pass needs none where its query is 0.

@@ -615,13 +615,16 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 64 
   // out is rounded, and with it Delta, by up to 2^-9 |dO| |out|. Over many keys
   // |out| is small beside the values and that is lost in dS's own rounding; a
   // row of few keys sums P (dP - Delta) over them, which is 0 for the exact
-  // Delta, first (9 x 9 causal: dq off by 0.30 % without, by 0.24 % with it).
-  // (Direct loads: these blocks have a few 16-key pieces in all.)
-  constexpr int kFewSteps = CAUSAL ? W / 2 + 1 : 2;
-  if (nsteps <= kFewSteps && q0 < a.nq) {
+  // Delta, first (9 x 9 causal: dq off by 0.30 % without, by 0.24 % with it; from
+  // 49 keys on by less than 0.25 % without). Causal, these are a head's first
+  // waves, else all of them: 2 x 2304 rows over 64 keys would take 61 us for 40,
+  // over 128 85 for 48.
+  constexpr int kFewKeys = CAUSAL ? 128 : 48;
+  const int64_t seen = CAUSAL ? min(nkb, q0 + 32 + shift) : nkb;
+  if (seen <= kFewKeys && q0 < a.nq) {
     float num[2] = {0.0f, 0.0f}, den[2] = {0.0f, 0.0f};
 #pragma unroll 2
-    for (int64_t key0 = 0; key0 < kend; key0 += 16) {
+    for (int64_t key0 = 0; key0 < seen; key0 += 16) {
       const int64_t ki = min(key0 + c16, nkb - 1);
       f32x4 s[2], g[2];
 #pragma unroll
